@@ -184,7 +184,7 @@ def prepare(case, seed):
             state["residual"] = torch.randn(m, n, device=DEVICE, generator=gen)
     if own:
         from flyweight_b200.kernels import int8
-        state["weight"] = int8.rows_int8(weight)         # laid out once, as a model's weights are
+        state["weight"] = int8.matrix_int8(weight)       # laid out once, as a model's weights are
     else:
         state["weight"] = _quantized(weight)
     return state
