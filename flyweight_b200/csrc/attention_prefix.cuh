@@ -1,0 +1,92 @@
+// What the kernels of attention over a shared prefix have in common: the batch as they see it.
+//
+// The tokens [group_start[g], group_start[g + 1]) belong to requests whose first group_pages[g] pages are the same ones;
+// the group's first token's block-table row names them.  A token sees the keys up to its own position: those of the shared
+// pages, then its request's own from position 64 * group_pages[g] on.
+#pragma once
+
+#include "common.cuh"
+
+namespace fwb {
+namespace prefix {
+
+constexpr int PAGE = 64;
+
+struct Batch {
+    const int* positions;        // [T]
+    const int* tok_seg;          // [T]
+    const int* block_table;      // [n_segments][max_pages]
+    const int* group_start;      // [n_groups + 1], rising
+    const int* group_pages;      // [n_groups]
+    int T, n_segments, n_groups, max_pages, num_pages;
+
+    __device__ __forceinline__ int start_of(int g) const {
+        const int t = group_start[g];
+        return t < 0 ? 0 : t > T ? T : t;
+    }
+    __device__ __forceinline__ int pages_of(int g) const {
+        const int n = group_pages[g];
+        return n < 0 ? 0 : n > max_pages ? max_pages : n;
+    }
+    // the block-table row of a token, null for a token of no request
+    __device__ __forceinline__ const int* row_of(int token) const {
+        const int seg = tok_seg[token];
+        return seg < 0 || seg >= n_segments ? nullptr : block_table + (size_t)seg * max_pages;
+    }
+    __device__ __forceinline__ bool is_page(int page) const { return page >= 0 && page < num_pages; }
+};
+
+// The token tile `index` when every group's tokens are cut into tiles of `per_tile`: its group, first token and tokens (0: no
+// such tile).  Asked by whole warps.
+struct TokenTile {
+    int group, first, count;
+};
+__device__ __forceinline__ TokenTile token_tile(const Batch& b, int index, int per_tile) {
+    const int lane = threadIdx.x & 31;
+    for (int g0 = 0; g0 < b.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        const int first = g < b.n_groups ? b.start_of(g) : 0;
+        int n = g < b.n_groups ? b.start_of(g + 1) - first : 0;
+        n = n < 0 ? 0 : n;
+        const int tiles = (n + per_tile - 1) / per_tile;
+        int upto = tiles;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, offset);
+            if (lane >= offset) upto += other;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, index < upto);
+        if (behind) {
+            const int owner = __ffs(behind) - 1;
+            const int inside = index - (__shfl_sync(0xffffffffu, upto, owner) - __shfl_sync(0xffffffffu, tiles, owner));
+            TokenTile t;
+            t.group = g0 + owner;
+            t.first = __shfl_sync(0xffffffffu, first, owner) + inside * per_tile;
+            const int left = __shfl_sync(0xffffffffu, n, owner) - inside * per_tile;
+            t.count = left < per_tile ? left : per_tile;
+            return t;
+        }
+        index -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return TokenTile{0, 0, 0};
+}
+// The most such tiles a batch can have, from what the host knows.
+inline long most_token_tiles(int T, int n_groups, int per_tile) {
+    const long most = ((long)T + (long)n_groups * (per_tile - 1)) / per_tile;
+    return most < T ? most : T;
+}
+
+// The group of a token, -1 for one behind the last group (or in front of the first).  Asked by whole warps.
+__device__ __forceinline__ int group_of(const Batch& b, int token) {
+    const int lane = threadIdx.x & 31;
+    int begun = 0;                                     // groups that start at or before the token
+    for (int g0 = 0; g0 <= b.n_groups; g0 += 32)
+        begun += __popc(__ballot_sync(0xffffffffu, g0 + lane <= b.n_groups && b.start_of(g0 + lane) <= token));
+    return begun > b.n_groups ? -1 : begun - 1;
+}
+
+// How a group's shared pages are cut into at most `splits` slices: pages a slice.
+__host__ __device__ __forceinline__ int pages_per_slice(int pages, int splits) { return (pages + splits - 1) / splits; }
+
+}  // namespace prefix
+}  // namespace fwb

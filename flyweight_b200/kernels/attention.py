@@ -264,3 +264,69 @@ def paged_attention(ctx, q, cache, block_table, n_heads, window, scale, out_dtyp
     return ops.attention_simt(q, k_pool, v_pool, batch.positions, batch.tok_seg, block_table,
                               n_heads, window, scale, out_dtype, sink=sink, softcap=softcap,
                               keep_first=keep_first)
+
+
+def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int) -> int:
+    """How many slices of a group's shared pages run as separate blocks."""
+    row_tiles = max(1, -(-n_tokens * group // 64)) * n_kv
+    return max(1, min(shared_pages, 64, -(-2 * SM_COUNT // row_tiles)))
+
+
+def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, group_start, group_pages, n_heads: int,
+                            scale: float, sink=None, softcap: float = 0.0, out=None, shared_pages=None, own_pages=None):
+    """Causal GQA of a batch whose requests share their first pages -- a system prompt, one prompt's many answers -- with
+    the shared keys and values read once for all requests of a group instead of once a request.
+
+    ``q`` [T][n_heads * head_dim], the pools [pages][kv_heads][64][head_dim] (all bf16 or all fp32), ``positions`` and
+    ``tok_seg`` [T], ``block_table`` [requests][pages] as in ``paged_attention``.  The tokens ``group_start[g]`` to
+    ``group_start[g + 1]`` (int32 [groups + 1], rising) are group g's; the block-table rows of its requests begin with the same
+    ``group_pages[g]`` pages (int32 [groups]; 0: nothing shared), named by the row of its first token.  Every token sees
+    the keys up to its position, in shared and own pages alike, whatever the number of tokens a request has in the step; the
+    result is ``paged_attention``'s.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
+    position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are in ``out``.
+
+    ``sink``: fp32 [n_heads], a score per head that joins every softmax denominator (not scaled, not capped, no value);
+    ``softcap`` > 0: scores become ``softcap * tanh(score / softcap)`` behind the scale.
+
+    All arrays are read on the device, so a captured step replays with other groups.  ``shared_pages`` and ``own_pages`` only
+    say what the work is cut for (the longest shared part, the longest own part; default: the block table's width)."""
+    from .lib import KernelError, c_float, check_tensor, is_bf16, ptr, stream
+    check_tensor("q", q)
+    check_tensor("k pool", k_pool, q.dtype)
+    check_tensor("v pool", v_pool, q.dtype, k_pool.shape)
+    if q.dim() != 2 or k_pool.dim() != 4 or k_pool.shape[2] != 64:
+        raise KernelError("q must be [tokens][heads * head_dim], the pools [pages][kv_heads][64][head_dim]")
+    num_pages, n_kv, _, head_dim = k_pool.shape
+    T = q.shape[0]
+    if n_heads <= 0 or n_heads % n_kv or q.shape[1] != n_heads * head_dim:
+        raise KernelError(f"q has {q.shape[1]} columns, expected {n_heads} heads of {head_dim} over {n_kv} KV heads")
+    if head_dim > 256:
+        raise KernelError(f"head sizes up to 256, got {head_dim}")
+    for name, tensor in (("positions", positions), ("tok_seg", tok_seg), ("block table", block_table),
+                         ("group starts", group_start), ("group pages", group_pages)):
+        check_tensor(name, tensor, torch.int32)
+    if positions.numel() < T or tok_seg.numel() < T:
+        raise KernelError(f"{T} tokens need a position and a request each")
+    if block_table.dim() != 2 or block_table.numel() == 0:
+        raise KernelError("the block table must be [requests][pages]")
+    groups = group_pages.numel()
+    if group_start.numel() != groups + 1:
+        raise KernelError(f"{groups} groups need {groups + 1} starts, got {group_start.numel()}")
+    if sink is not None:
+        check_tensor("sink", sink, torch.float32, (n_heads,))
+    if not softcap >= 0:
+        raise KernelError("a soft-cap must not be negative")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        check_tensor("attention output", out, q.dtype, q.shape)
+    if T == 0 or groups == 0:
+        return out
+    width = block_table.shape[1]
+    splits = shared_prefix_splits(T, n_kv, n_heads // n_kv, min(width, width if shared_pages is None else max(1, shared_pages)))
+    part_o = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
+    part_ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
+    lib.call("fwb_attention_prefix", ptr(q), ptr(k_pool), ptr(v_pool), is_bf16(q), ptr(positions), ptr(tok_seg), ptr(block_table),
+             block_table.shape[0], width, num_pages, ptr(group_start), ptr(group_pages), groups, ptr(part_o), ptr(part_ml),
+             ptr(out), T, n_heads, n_kv, head_dim, splits, c_float(scale), ptr(sink), c_float(softcap), stream(), launches=2)
+    return out

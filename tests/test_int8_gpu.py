@@ -1,0 +1,257 @@
+"""The 8-bit products and the kernels that make their operands, against the definitions in 64 bits.
+
+The integer sums are exact, so a product has three or four fp32 roundings (2^-24 each, half a step) and the output's: half a step
+of bfloat16 is 2^-8.  The rows' integers are compared for equality; behind a norm, whose fp32 value is a few roundings off,
+an integer may be the neighbour where the quotient lies that near to a half."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F64 = torch.float64
+HALF = 2.0 ** -24
+HALF_BF16 = 2.0 ** -8
+
+
+@pytest.fixture(autouse=True)
+def guard_bands():
+    from gpu_util import GuardedOutputs
+    with GuardedOutputs() as guard:
+        yield guard
+        guard.check()
+        guard.forget()
+
+
+def rows_of(R, K, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, K, generator=g) * torch.exp(torch.randn(R, 1, generator=g))
+    x[:, :: max(1, K // 3)] *= 9.0
+    return x.to(dtype)
+
+
+def define(x):
+    """Integers and scales by the definition, on the CPU in 64 bits (the scale is a 32-bit number)."""
+    wide = x.to(F64)
+    scale = (wide.abs().amax(dim=1) / 127).to(torch.float32)
+    values = torch.where(scale[:, None] > 0, wide / scale.to(F64)[:, None], torch.zeros_like(wide)).round()
+    return values.clamp(-127, 127), scale
+
+
+def check_layout(q, R, K):
+    assert q.shape == (R, K) and q.values.shape == (R, (K + 15) // 16 * 16) and q.values.dtype == torch.int8
+    assert not q.values[:, K:].any(), "columns behind the last one must be zero"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,K", [(1, 1), (3, 7), (1, 16), (5, 100), (2, 2047), (17, 2048), (4, 8192), (3, 10001), (300, 64),
+                                 (1, 131071)])
+def test_rows_become_the_defined_integers(R, K, dtype):
+    from flyweight_b200.kernels import int8
+    x = rows_of(R, K, dtype)
+    got = int8.rows_int8(x.to(DEV))
+    check_layout(got, R, K)
+    values, scale = define(x)
+    assert torch.equal(got.scales.cpu(), scale)
+    assert torch.equal(got.values[:, :K].cpu().to(F64), values)
+    assert torch.equal(got.float().cpu(), (values * scale.to(F64)[:, None]).float())
+
+
+def test_ties_go_to_the_even_integer():
+    from flyweight_b200.kernels import int8
+    # the scale is exactly 1: halves are exact ties
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 63.5, 64.5, -125.5, 126.5, 0.0]])
+    got = int8.rows_int8(x.to(DEV)).values[0, :12].tolist()
+    assert got == [127, 0, 2, 2, 0, -2, -2, 64, 64, -126, 126, 0]
+    # next to a tie by one step of fp32, on both sides
+    up, down = math.nextafter(2.5, 3), math.nextafter(2.5, 2)
+    near = torch.tensor([[127.0, 2.5 + 2.0 ** -22, 2.5 - 2.0 ** -22, -2.5 - 2.0 ** -22, -2.5 + 2.0 ** -22, 100.5 + 2.0 ** -17]])
+    assert up > 2.5 > down
+    assert int8.rows_int8(near.to(DEV)).values[0, :6].tolist() == [127, 3, 2, -3, -2, 101]
+
+
+def test_many_values_next_to_a_half():
+    """Scales that are no power of two, values placed on and around every half: the quotient's own rounding decides."""
+    from flyweight_b200.kernels import int8
+    g = torch.Generator().manual_seed(3)
+    top = torch.rand(64, 1, generator=g) * 3 + 0.1
+    scale = (top.to(F64) / 127).to(torch.float32)
+    halves = torch.arange(-126, 126).to(F64) + 0.5
+    x = (halves[None, :] * scale.to(F64)).to(torch.float32)
+    x = torch.cat([top, x, torch.nextafter(x, torch.full_like(x, 9.0)), torch.nextafter(x, torch.full_like(x, -9.0))], dim=1)
+    values, want_scale = define(x)
+    got = int8.rows_int8(x.to(DEV))
+    assert torch.equal(got.scales.cpu(), want_scale)
+    assert torch.equal(got.values[:, :x.shape[1]].cpu().to(F64), values)
+
+
+def test_rows_of_zeros_infinities_and_nan():
+    from flyweight_b200.kernels import int8
+    x = rows_of(6, 200, torch.float32)
+    x[1] = 0.0
+    x[2, 5] = math.inf
+    x[3, 199] = math.nan
+    x[4, 0] = -math.inf
+    got = int8.rows_int8(x.to(DEV))
+    scales = got.scales.cpu()
+    assert scales[1] == 0 and not got.values[1].any()
+    assert torch.isnan(scales[[2, 3, 4]]).all() and torch.isfinite(scales[[0, 1, 5]]).all()
+    w = int8.matrix_int8(rows_of(40, 200, torch.bfloat16, 1).to(DEV))
+    y = int8.linear_int8(got, w, torch.float32).cpu()
+    assert torch.isnan(y[[2, 3, 4]]).all() and torch.isfinite(y[[0, 5]]).all() and not y[1].any()
+
+
+@pytest.mark.parametrize("R,K", [(1, 64), (7, 100), (3, 2048), (33, 2047), (2, 8200)])
+@pytest.mark.parametrize("with_delta", [False, True])
+def test_normed_rows(R, K, with_delta):
+    from flyweight_b200.kernels import int8
+    g = torch.Generator().manual_seed(5)
+    x, w = rows_of(R, K, torch.float32), 1 + 0.2 * torch.randn(K, generator=g)
+    delta = torch.randn(R, K, generator=g) if with_delta else None
+    held = x.to(DEV)
+    got = int8.rmsnorm_int8(held, w.to(DEV), 1e-5, delta=None if delta is None else delta.to(DEV))
+    check_layout(got, R, K)
+    summed = x if delta is None else x + delta
+    assert torch.equal(held.cpu(), summed)
+    wide = summed.to(F64)
+    y = wide / torch.sqrt((wide * wide).mean(dim=1, keepdim=True) + 1e-5) * w.to(F64)
+    # squares: a product and K/2048 + 16 additions deep at most; mean, eps, root, reciprocal; two products
+    off = (K / 2048 + 16 + 8) * HALF
+    scale = y.abs().amax(dim=1) / 127
+    assert ((got.scales.cpu().to(F64) - scale).abs() <= scale * (off + 2 * HALF)).all()
+    quotient = y / got.scales.cpu().to(F64)[:, None]
+    assert ((got.values[:, :K].cpu().to(F64) - quotient).abs() <= 0.5 + 127 * 2 * off).all()
+
+
+def test_normed_rows_of_an_index():
+    from flyweight_b200.kernels import int8
+    x, w = rows_of(9, 96, torch.float32).to(DEV), torch.ones(96, device=DEV)
+    rows = torch.tensor([4, 4, 0, 8], dtype=torch.int32, device=DEV)
+    some, every = int8.rmsnorm_int8(x, w, 1e-5, rows=rows), int8.rmsnorm_int8(x, w, 1e-5)
+    assert torch.equal(some.values, every.values[rows.long()]) and torch.equal(some.scales, every.scales[rows.long()])
+
+
+# tokens, columns, features: one token to a prompt, sizes that fill no tile on either side of every choice of kernel
+PRODUCTS = [(1, 16, 8), (1, 2048, 2048), (2, 100, 33), (3, 4097, 130), (7, 1, 5), (8, 2048, 1024), (9, 640, 257), (16, 1024, 4608),
+            (17, 512, 129), (24, 96, 300), (31, 1040, 1000), (33, 200, 64), (64, 4096, 512), (65, 129, 260), (100, 48, 1),
+            (129, 300, 385), (200, 1024, 640), (257, 257, 257), (513, 2048, 768), (700, 100, 1030), (1100, 512, 520)]
+
+
+@pytest.mark.parametrize("M,K,N", PRODUCTS)
+@pytest.mark.parametrize("form", ["fp32", "bf16", "add", "in place"])
+def test_product(M, K, N, form):
+    from flyweight_b200.kernels import int8
+    x, w = rows_of(M, K, torch.bfloat16, 1), rows_of(N, K, torch.bfloat16, 2)
+    rows, matrix = int8.rows_int8(x.to(DEV)), int8.matrix_int8(w.to(DEV))
+    (xq, xs), (wq, ws) = define(x), define(w)
+    want = (xq @ wq.T) * xs.to(F64)[:, None] * ws.to(F64)[None, :]
+    bound = want.abs() * 3 * HALF * 1.01 + 2.0 ** -148
+    if form in ("fp32", "bf16"):
+        got = int8.linear_int8(rows, matrix, torch.float32 if form == "fp32" else torch.bfloat16)
+        if form == "bf16":
+            bound = bound + want.abs() * HALF_BF16 * 1.001
+    else:
+        addend = torch.randn(M, N, generator=torch.Generator().manual_seed(9))
+        held = addend.to(DEV)
+        got = int8.linear_int8(rows, matrix, torch.float32, addend=held, out=held if form == "in place" else None)
+        assert form != "in place" or got is held
+        want = want + addend.to(F64)
+        bound = bound + want.abs() * HALF * 1.01
+    assert got.shape == (M, N)
+    assert ((got.cpu().to(F64) - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 300])
+def test_a_row_does_not_depend_on_the_others(M):
+    """Exact sums and one order of the scales: the bits of a row are the same in every batch, so in every kernel."""
+    from flyweight_b200.kernels import int8
+    x, matrix = rows_of(600, 1000, torch.bfloat16).to(DEV), int8.matrix_int8(rows_of(700, 1000, torch.bfloat16, 1).to(DEV))
+    every, some = int8.linear_int8(x, matrix, torch.float32), int8.linear_int8(x[:M], matrix, torch.float32)
+    assert torch.equal(every[:M], some)
+
+
+def test_the_largest_integers_do_not_overflow():
+    from flyweight_b200.kernels import int8
+    K = int8.MAX_COLUMNS
+    x = torch.ones(2, K, dtype=torch.bfloat16, device=DEV)
+    x[1] = -1.0
+    got = int8.linear_int8(x, int8.matrix_int8(torch.ones(3, K, dtype=torch.bfloat16, device=DEV)), torch.float32).cpu()
+    scale = torch.tensor(1 / 127, dtype=F64).float().to(F64)
+    want = 127.0 * 127.0 * K * scale * scale
+    assert ((got.to(F64)[0] - want).abs() <= want * 4 * HALF).all() and torch.equal(got[1], -got[0])
+
+
+def test_inputs_in_32_bits_are_brought_to_integers_first():
+    from flyweight_b200.kernels import int8
+    for M in (1, 6, 130):
+        x, matrix = rows_of(M, 333, torch.float32).to(DEV), int8.matrix_int8(rows_of(50, 333, torch.float32, 1).to(DEV))
+        assert torch.equal(int8.linear_int8(x, matrix, torch.bfloat16), int8.linear_int8(int8.rows_int8(x), matrix, torch.bfloat16))
+
+
+def gated(act, limit, g, u):
+    if act == "silu":
+        return g / (1 + torch.exp(-g)) * u
+    if act == "gelu_tanh":
+        # 0.5 (1 + tanh(a)) = 1 / (1 + e^(-2 a)), without the cancellation
+        return g / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3))) * u
+    if act == "relu":
+        return g.clamp(min=0) * u
+    g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+    return g / (1 + torch.exp(-1.702 * g)) * (u + 1)
+
+
+@pytest.mark.parametrize("M,K,F", [(1, 64, 16), (1, 2048, 1000), (5, 100, 33), (8, 2048, 512), (16, 512, 130), (20, 600, 257),
+                                   (48, 300, 96), (64, 2048, 640), (130, 257, 65), (300, 1024, 400), (520, 512, 1000)])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "relu", "swish_clamped"])
+def test_gated_product(M, K, F, act):
+    from flyweight_b200.kernels import int8
+    x, w = rows_of(M, K, torch.bfloat16, 1), rows_of(2 * F, K, torch.bfloat16, 2) * K ** -0.5
+    limit = 3.0 if act == "swish_clamped" else 0.0
+    got = int8.gated_int8(x.to(DEV), int8.matrix_int8(w.to(DEV)), activation=act, limit=limit)
+    (xq, xs), (wq, ws) = define(x), define(w)
+    y = (xq @ wq.T) * xs.to(F64)[:, None] * ws.to(F64)[None, :]
+    want = gated(act, limit, y[:, :F], y[:, F:])
+    # the output's rounding; in front of it fp32: the exponent's argument is a few roundings of itself off (|z| up to 88), the
+    # hardware exponential and quotient a few more.  From 1 + e^-z = 2^126 on the hardware quotient is 0 where the value is
+    # g u 2^-126 at most: an absolute part of that size, which the first run of this test did not allow for
+    bound = want.abs() * (HALF_BF16 * 1.001 + 2.0 ** -13) + (y[:, :F] * (y[:, F:].abs() + 1)).abs() * 2.0 ** -125
+    if act == "swish_clamped":
+        # u + 1 next to u = -1: u itself is three half steps off, the sum one more, of at most (limit + 1), times the swish of g
+        g = y[:, :F].clamp(max=limit)
+        bound += (g / (1 + torch.exp(-1.702 * g))).abs() * (limit + 1) * 4 * HALF
+    assert got.dtype == torch.bfloat16 and got.shape == (M, F)
+    assert ((got.cpu().to(F64) - want).abs() <= bound).all()
+
+
+def test_no_rows_at_all():
+    from flyweight_b200.kernels import int8
+    matrix = int8.matrix_int8(rows_of(40, 64, torch.bfloat16).to(DEV))
+    none = torch.empty((0, 64), dtype=torch.bfloat16, device=DEV)
+    assert int8.rows_int8(none).shape == (0, 64)
+    assert int8.linear_int8(none, matrix, torch.float32).shape == (0, 40)
+    assert int8.gated_int8(none, matrix).shape == (0, 20)
+
+
+def test_refusals():
+    from flyweight_b200.kernels import KernelError, int8
+    x, w = rows_of(4, 64, torch.bfloat16).to(DEV), rows_of(10, 64, torch.bfloat16).to(DEV)
+    matrix, rows = int8.matrix_int8(w), int8.rows_int8(x)
+    for call in (lambda: int8.rows_int8(x.to(torch.float16)), lambda: int8.rows_int8(x.t()), lambda: int8.rows_int8(x[0]),
+                 lambda: int8.rows_int8(torch.empty((2, int8.MAX_COLUMNS + 1), dtype=torch.bfloat16, device=DEV)),
+                 lambda: int8.rows_int8(torch.empty((2, 0), dtype=torch.bfloat16, device=DEV)),
+                 lambda: int8.linear_int8(rows, w, torch.float32), lambda: int8.linear_int8(rows, rows, torch.float32),
+                 lambda: int8.linear_int8(rows, matrix, torch.float16),
+                 lambda: int8.linear_int8(x[:, :32].contiguous(), matrix, torch.float32),
+                 lambda: int8.linear_int8(rows, matrix, torch.bfloat16, addend=torch.zeros(4, 10, device=DEV)),
+                 lambda: int8.linear_int8(rows, matrix, torch.float32, addend=torch.zeros(4, 9, device=DEV)),
+                 lambda: int8.linear_int8(rows, matrix, torch.float32, out=torch.zeros(3, 10, device=DEV)),
+                 lambda: int8.gated_int8(rows, matrix, activation="tanh"),
+                 lambda: int8.gated_int8(rows, int8.matrix_int8(w[:9].contiguous())),
+                 lambda: int8.rmsnorm_int8(x, torch.ones(64, device=DEV), 1e-5),
+                 lambda: int8.rmsnorm_int8(x.float(), torch.ones(63, device=DEV), 1e-5),
+                 lambda: int8.rmsnorm_int8(x.float(), torch.ones(64, device=DEV), 1e-5, delta=x.float(),
+                                           rows=torch.zeros(1, dtype=torch.int32, device=DEV))):
+        with pytest.raises(KernelError):
+            call()
