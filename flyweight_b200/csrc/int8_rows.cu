@@ -4,19 +4,24 @@
 //
 // with y the rows themselves or their RMS norm, y = (x r) w, r = 1 / sqrt(mean(x^2) + eps), behind a residual sum
 // x += delta where there is one.  The quotient's rounding is the exact one: a product with 1 / s decides all but the values
-// next to a half, and there the sign of x - (n +- 1/2) s, which one fused multiply-add gives without an error, decides.
-// A row of zeros has the scale 0.  A row that holds an infinity or a NaN has the scale NaN (and integers 0): whatever is
-// made of it is NaN.
+// next to a half (it is off by 127 * 2^-23 at most), and there the remainder decides.  A row of zeros has the scale 0.  A row that holds an infinity or a NaN has the scale NaN:
+// whatever is made of it is NaN.
 //
 // Rows of integers lie `stride` bytes apart, a multiple of 16 (what TMA asks of a row), and are zero behind column K.
+//
+// Bound by memory.  A row is read once and held in registers between its passes (rows of more than 16,384 are read again).
+// Many rows: a warp has up to 2,048 columns of one, so that as much as possible is on the way at once and nobody waits at
+// a barrier; few: a block has a row, a thread eight columns, for the shortest way through.  Rounding by adding 1.5 * 2^23, whose
+// low byte is the integer: the conversion instructions have a quarter of the adders' rate.
 #include "common.cuh"
 
 using namespace fwb;
 
 namespace {
 
-constexpr int THREADS = 256;
 constexpr int CHUNK = 8;                 // elements a thread takes at once
+constexpr int WARP_ROWS = 4;             // warps of a block whose warps have a row each
+constexpr float TINY_ROW = 1e-30f;       // a row without a larger value is taken as zeros: its scale would be no normal number
 
 struct RowsInt8Params {
     const void* x;               // [.][K] bf16 or fp32
@@ -30,109 +35,223 @@ struct RowsInt8Params {
     int vector;                  // rows start on 16-byte borders and K is a multiple of 8
 };
 
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int k, int K, int vector, float (&v)[CHUNK]) {
+// Eight elements of a row as they lie in memory, zeros behind its end.
+template <typename T> struct Raw;
+template <> struct Raw<float> { float4 a, b; };
+template <> struct Raw<__nv_bfloat16> { uint4 a; };
+__device__ __forceinline__ void load(Raw<float>& to, const float* row, int k, int K, int vector) {
     if (vector) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(row + k);
-            const uint32_t p[4] = {a.x, a.y, a.z, a.w};
+        to.a = *reinterpret_cast<const float4*>(row + k), to.b = *reinterpret_cast<const float4*>(row + k + 4);
+    } else {
+        float v[CHUNK];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(p[i] << 16);
-                v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+        for (int i = 0; i < CHUNK; ++i) v[i] = k + i < K ? row[k + i] : 0.0f;
+        to.a = make_float4(v[0], v[1], v[2], v[3]), to.b = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+__device__ __forceinline__ void load(Raw<__nv_bfloat16>& to, const __nv_bfloat16* row, int k, int K, int vector) {
+    if (vector) to.a = *reinterpret_cast<const uint4*>(row + k);
+    else {
+        uint32_t v[CHUNK];
+        const unsigned short* at = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) v[i] = k + i < K ? at[k + i] : 0;
+        to.a = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
+}
+__device__ __forceinline__ void values(const Raw<float>& r, float (&v)[CHUNK]) {
+    v[0] = r.a.x, v[1] = r.a.y, v[2] = r.a.z, v[3] = r.a.w, v[4] = r.b.x, v[5] = r.b.y, v[6] = r.b.z, v[7] = r.b.w;
+}
+__device__ __forceinline__ void values(const Raw<__nv_bfloat16>& r, float (&v)[CHUNK]) {
+    const uint32_t p[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(p[i] << 16);
+        v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+    }
+}
+
+// Eight values' integers.
+//
+// Checked: n = x (1 / s) rounded is the integer or its neighbour; e = x - n s has no rounding error (a multiple of the smaller
+// of x's and s's last places, and at most about s / 2), so |e| against s / 2 tells.
+//
+// Not checked, for values of eight bits under a maximum m of eight bits (bfloat16 rows): 254 |x| / m is an odd integer, and x / (m / 127)
+// a tie, or it is 2^-8 or more away from one.  s is m / 127 rounded, so the ties all lie on one side of their halves, by 2^-24 of
+// themselves at most; `inv` is 1 / s moved by 2^-22 of itself towards that side, which decides every tie and nothing else.
+template <bool CHECKED>
+__device__ __forceinline__ uint2 quantize(const float (&v)[CHUNK], float s, float inv) {
+    constexpr float ROUND = 12582912.0f;               // 1.5 * 2^23
+    uint32_t word[CHUNK];
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CHUNK; ++i) {
+        const float n = fmaf(v[i], inv, ROUND);
+        word[i] = __float_as_uint(n);
+        if (CHECKED) off = fmaxf(off, fabsf(fmaf(-__fsub_rn(n, ROUND), s, v[i])));
+    }
+    const float half = 0.5f * s;
+    if (CHECKED && off >= half) {
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) {
+            const float n = __uint_as_float(word[i]), e = fmaf(-__fsub_rn(n, ROUND), s, v[i]);
+            if (fabsf(e) > half || (fabsf(e) == half && (word[i] & 1))) word[i] += e > 0.0f ? 1 : -1;
+        }
+    }
+    uint2 packed;
+    packed.x = __byte_perm(__byte_perm(word[0], word[1], 0x0040), __byte_perm(word[2], word[3], 0x0040), 0x5410);
+    packed.y = __byte_perm(__byte_perm(word[4], word[5], 0x0040), __byte_perm(word[6], word[7], 0x0040), 0x5410);
+    return packed;
+}
+
+// What the threads of a row hold, put together; every one of them gets the result.
+template <bool WARP>
+__device__ __forceinline__ unsigned row_max(unsigned v, unsigned* scratch) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    return __reduce_max_sync(0xffffffffu, scratch[lane < warps ? lane : 0]);
+}
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+    v = warp_sum(v);
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    return warp_sum(lane < warps ? scratch[lane] : 0.0f);
+}
+
+enum Form : int { PLAIN = 0, NORM = 1, NORM_DELTA = 2 };
+
+__device__ __forceinline__ void keep(Raw<float>& r, const float (&v)[CHUNK]) {
+    r.a = make_float4(v[0], v[1], v[2], v[3]), r.b = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void keep(Raw<__nv_bfloat16>&, const float (&)[CHUNK]) {}
+
+// WARP: a warp has a row (else the block).  CHUNKS: eight-element pieces a thread holds; 0: rows of any length, read again in
+// every pass.
+template <typename T, int FORM, bool WARP, int CHUNKS>
+__global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : CHUNKS == 8 ? 256 : 1024) rows_int8_kernel(const RowsInt8Params prm) {
+    constexpr int HELD = CHUNKS ? CHUNKS : 1;
+    __shared__ float sums[32];
+    __shared__ unsigned tops[32];
+    const int K = prm.K, step = (WARP ? 32 : blockDim.x) * CHUNK, k0 = (WARP ? threadIdx.x & 31 : threadIdx.x) * CHUNK;
+    pdl_entry();
+    const int r = WARP ? blockIdx.x * WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP && r >= prm.R) return;
+    const T* row = reinterpret_cast<const T*>(prm.x) + (prm.rows ? (size_t)prm.rows[r] : (size_t)r) * K;
+    Raw<T> raw[HELD];
+    if constexpr (CHUNKS > 0) {
+#pragma unroll
+        for (int c = 0; c < HELD; ++c)
+            if (k0 + c * step < K) load(raw[c], row, k0 + c * step, K, prm.vector);
+    }
+    // visit(k, values): every chunk of this thread's; what it leaves in the values stays (fp32 rows that are held)
+    auto each = [&](auto&& visit) {
+        float v[CHUNK];
+        if constexpr (CHUNKS > 0) {
+#pragma unroll
+            for (int c = 0; c < HELD; ++c)
+                if (k0 + c * step < K) {
+                    values(raw[c], v);
+                    visit(k0 + c * step, v);
+                    if (FORM != PLAIN) keep(raw[c], v);
+                }
+        } else {
+            for (int k = k0; k < K; k += step) {
+                load(raw[0], row, k, K, prm.vector);
+                values(raw[0], v);
+                visit(k, v);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) v[i] = k + i < K ? to_f32(row[k + i]) : 0.0f;
-    }
-}
-
-__device__ __forceinline__ int quantize(float x, float s, float inv) {
-    const float t = x * inv;
-    float n = rintf(t);
-    if (fabsf(fabsf(t - n) - 0.5f) < 1e-4f) {          // next to a half: 127 * 2^-23 is far less than this
-        const float up = fmaf(-(n + 0.5f), s, x), down = fmaf(-(n - 0.5f), s, x);
-        const bool odd = ((int)n) & 1;
-        if (up > 0.0f || (up == 0.0f && odd)) n += 1.0f;
-        else if (down < 0.0f || (down == 0.0f && odd)) n -= 1.0f;
-    }
-    return (int)fminf(fmaxf(n, -127.0f), 127.0f);      // (a NaN comes out as a number)
-}
-
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    v = warp_max(v);
-    __syncthreads();
-    if (lane == 0) scratch[warp] = v;
-    __syncthreads();
-    v = scratch[lane < (int)(blockDim.x >> 5) ? lane : 0];
-    return warp_max(v);
-}
-
-// A block a row; every pass reads the row again (it lies in L1 or L2 by then).
-template <typename T, bool NORM>
-__global__ void __launch_bounds__(THREADS) rows_int8_kernel(const RowsInt8Params prm) {
-    __shared__ float scratch[33];
-    pdl_entry();
-    const int r = blockIdx.x, K = prm.K;
-    const size_t source = prm.rows ? (size_t)prm.rows[r] : (size_t)r;
-    const T* row = reinterpret_cast<const T*>(prm.x) + source * K;
+    };
     float inv_rms = 1.0f;
-    if constexpr (NORM) {
+    if constexpr (FORM != PLAIN) {
         float square = 0.0f;
-        for (int k = threadIdx.x * CHUNK; k < K; k += THREADS * CHUNK) {
-            float v[CHUNK];
-            load_chunk(row, k, K, prm.vector, v);
-            if (prm.delta) {
+        each([&](int k, float (&v)[CHUNK]) {
+            if constexpr (FORM == NORM_DELTA) {
+                Raw<float> more;
                 float d[CHUNK];
-                load_chunk(prm.delta + source * K, k, K, prm.vector, d);
-                float* at = const_cast<float*>(reinterpret_cast<const float*>(row));
+                load(more, prm.delta + (size_t)r * K, k, K, prm.vector);
+                values(more, d);
+                float* at = const_cast<float*>(reinterpret_cast<const float*>(row)) + k;       // the residual sum, in place
 #pragma unroll
-                for (int i = 0; i < CHUNK; ++i) {
-                    v[i] += d[i];
-                    if (k + i < K) at[k + i] = v[i];
+                for (int i = 0; i < CHUNK; ++i) v[i] += d[i];
+                if (prm.vector) {
+                    *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < CHUNK; ++i)
+                        if (k + i < K) at[i] = v[i];
                 }
             }
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i) square = fmaf(v[i], v[i], square);
-        }
-        inv_rms = 1.0f / sqrtf(block_sum(square, scratch) / (float)K + prm.eps);
+        });
+        inv_rms = 1.0f / sqrtf(row_sum<WARP>(square, sums) / (float)K + prm.eps);
     }
-    auto value = [&](int k, float (&v)[CHUNK]) {
-        load_chunk(row, k, K, prm.vector, v);
-        if constexpr (NORM) {
-            float w[CHUNK];
-            load_chunk(prm.norm_w, k, K, prm.vector, w);
+    auto finish_norm = [&](int k, float (&v)[CHUNK]) {
+        Raw<float> more;
+        float gain[CHUNK];
+        load(more, prm.norm_w, k, K, prm.vector);
+        values(more, gain);
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) v[i] = (v[i] * inv_rms) * w[i];
-        }
+        for (int i = 0; i < CHUNK; ++i) v[i] = (v[i] * inv_rms) * gain[i];
     };
-    float most = 0.0f, bad = 0.0f;
-    for (int k = threadIdx.x * CHUNK; k < K; k += THREADS * CHUNK) {
-        float v[CHUNK];
-        value(k, v);
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            most = fmaxf(most, fabsf(v[i]));
-            bad += v[i] * 0.0f;                        // NaN where v is none or no finite number
-        }
-    }
-    most = block_max(bad != bad ? INFINITY : most, scratch);
-    const float s = most / 127.0f, inv = most < 1e-30f || most > 3e38f ? 0.0f : 1.0f / s;
-    if (threadIdx.x == 0) prm.scales[r] = most > 3.402823466e38f ? __int_as_float(0x7fffffff) : (most < 1e-30f ? 0.0f : s);
-    for (int k = threadIdx.x * CHUNK; k < prm.stride; k += THREADS * CHUNK) {
-        float v[CHUNK] = {};
-        if (k < K) value(k, v);
-        uint32_t word[2] = {0, 0};
+    // magnitudes as bits: in their order infinity lies above every number and NaN above infinity
+    unsigned top = 0;
+    each([&](int k, float (&v)[CHUNK]) {
+        if (FORM != PLAIN) finish_norm(k, v);
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i)
-            if (k + i < K) word[i >> 2] |= (uint32_t)(quantize(v[i], s, inv) & 0xff) << (8 * (i & 3));
-        *reinterpret_cast<uint2*>(prm.q + (size_t)r * prm.stride + k) = make_uint2(word[0], word[1]);
-    }
+            if (FORM == PLAIN || prm.vector || k + i < K) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    });
+    top = row_max<WARP>(top, tops);
+    const float most = __uint_as_float(top), s = most / 127.0f;
+    const bool finite = top < 0x7f800000u, zero = most < TINY_ROW;
+    float inv = !finite || zero ? 0.0f : 1.0f / s;
+    // which side of its half a tie of a bfloat16 row lies on: s above m / 127, towards zero; s below, away from it
+    const float above = fmaf(s, 127.0f, -most);
+    const bool sided = sizeof(T) == 2 && above != 0.0f;
+    if (sided) inv = fmaf(inv, above > 0.0f ? -0x1p-22f : 0x1p-22f, inv);
+    if (k0 == 0) prm.scales[r] = !finite ? __int_as_float(0x7fffffff) : zero ? 0.0f : s;
+    signed char* out = prm.q + (size_t)r * prm.stride;
+    each([&](int k, float (&v)[CHUNK]) {
+        if (FORM != PLAIN && CHUNKS == 0) finish_norm(k, v);
+        uint2 packed = sided ? quantize<false>(v, s, inv) : quantize<true>(v, s, inv);
+        if (inv == 0.0f) packed = make_uint2(0, 0);
+        if (FORM != PLAIN && !prm.vector && k + CHUNK > K) {           // what a norm made of columns that are none
+            const unsigned long long mask = ~0ull >> (8 * (k + CHUNK - K));
+            packed.x &= (uint32_t)mask, packed.y &= (uint32_t)(mask >> 32);
+        }
+        *reinterpret_cast<uint2*>(out + k) = packed;
+    });
+    // from the last chunk to the stride: at most one piece of eight
+    if (k0 == 0 && ((K + 7) & ~7) < prm.stride) *reinterpret_cast<uint2*>(out + ((K + 7) & ~7)) = make_uint2(0, 0);
+}
+
+template <typename T, int FORM, bool WARP, int CHUNKS>
+void launch(const RowsInt8Params& prm, int threads, cudaStream_t stream) {
+    fwb::pdl(rows_int8_kernel<T, FORM, WARP, CHUNKS>, WARP ? (prm.R + WARP_ROWS - 1) / WARP_ROWS : prm.R, threads, 0, stream)(prm);
+}
+
+// (2,048 columns of bf16, us: 1,000 rows by blocks 3.4; 1,200 rows by warps 5.5; 8,192 rows by warps 15.2, by blocks 22)
+constexpr int MANY_ROWS = 148 * 16;
+template <typename T, int FORM>
+void launch(const RowsInt8Params& prm, cudaStream_t stream) {
+    const int pieces = (prm.K + CHUNK - 1) / CHUNK;
+    const bool many = prm.R >= MANY_ROWS;
+    if (pieces <= 32) launch<T, FORM, true, 1>(prm, 32 * WARP_ROWS, stream);
+    else if (many && pieces <= 128) launch<T, FORM, true, 4>(prm, 32 * WARP_ROWS, stream);
+    else if (many && pieces <= 256) launch<T, FORM, true, 8>(prm, 32 * WARP_ROWS, stream);
+    else if (many && pieces <= 2048) launch<T, FORM, false, 8>(prm, pieces <= 512 ? 64 : pieces <= 1024 ? 128 : 256, stream);
+    else if (pieces <= 1024) launch<T, FORM, false, 1>(prm, (pieces + 31) / 32 * 32, stream);
+    else if (pieces <= 2048) launch<T, FORM, false, 2>(prm, 1024, stream);
+    else launch<T, FORM, false, 0>(prm, 1024, stream);
 }
 
 }  // namespace
@@ -147,8 +266,9 @@ FWB_API int fwb_rows_int8(const void* x, int x_bf16, const float* delta, const f
     RowsInt8Params prm{x, delta, norm_w, rows, (signed char*)q, scales, R, K, stride, eps, 0};
     const uintptr_t bits = (uintptr_t)x | (uintptr_t)delta | (uintptr_t)norm_w;
     prm.vector = (K & 7) == 0 && (bits & 15) == 0;
-    if (norm_w) fwb::pdl(rows_int8_kernel<float, true>, R, THREADS, 0, stream)(prm);
-    else if (x_bf16) fwb::pdl(rows_int8_kernel<__nv_bfloat16, false>, R, THREADS, 0, stream)(prm);
-    else fwb::pdl(rows_int8_kernel<float, false>, R, THREADS, 0, stream)(prm);
+    if (delta) launch<float, NORM_DELTA>(prm, stream);
+    else if (norm_w) launch<float, NORM>(prm, stream);
+    else if (x_bf16) launch<__nv_bfloat16, PLAIN>(prm, stream);
+    else launch<float, PLAIN>(prm, stream);
     return fwb_launch_status();
 }

@@ -16,22 +16,39 @@ from typing import Optional, Union
 import torch
 
 from . import lib
-from .lib import KernelError, c_float, check_tensor, is_bf16, ptr, stream
+from .lib import KernelError, check_tensor
+from .ops import GATE_ACTIVATIONS
 
 MAX_COLUMNS = 131071          # 128 * 128 * K stays below 2^31
+_FP32, _BF16 = torch.float32, torch.bfloat16
 
 
 class Int8Rows:
-    """Rows of integers: ``values`` int8 [R][stride], zero from column ``columns`` on (``stride``: the next multiple of 16),
-    ``scales`` fp32 [R]; element (r, k) stands for ``values[r, k] * scales[r]``."""
-    __slots__ = ("values", "scales", "columns")
+    """Rows of integers with a scale each: element (r, k) stands for ``values[r, k] * scales[r]``.  ``values``: int8 [R][stride],
+    zero from column ``columns`` on (``stride``: the next multiple of 16); ``scales``: fp32 [R].  One buffer holds both."""
+    __slots__ = ("_buffer", "_rows", "columns", "_stride", "_address", "_scales")
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor, columns: int):
-        self.values, self.scales, self.columns = values, scales, columns
+    def __init__(self, buffer: torch.Tensor, rows: int, columns: int):
+        self._buffer, self._rows, self.columns = buffer, rows, columns
+        self._stride = (columns + 15) & ~15
+        self._address = buffer.data_ptr()
+        self._scales = self._address + rows * self._stride
 
     @property
     def shape(self):
-        return (self.values.shape[0], self.columns)
+        return (self._rows, self.columns)
+
+    @property
+    def device(self):
+        return self._buffer.device
+
+    @property
+    def values(self) -> torch.Tensor:
+        return self._buffer[:self._rows * self._stride].view(torch.int8).view(self._rows, self._stride)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._buffer[self._rows * self._stride:].view(_FP32)
 
     def float(self) -> torch.Tensor:
         """What the integers stand for, fp32 [R][columns]."""
@@ -43,40 +60,49 @@ class Int8Matrix(Int8Rows):
     __slots__ = ()
 
 
-def _quantize(x: torch.Tensor, delta, norm, rows, eps: float, kind):
-    K = x.shape[-1]
+def _input(name: str, x: torch.Tensor) -> int:
+    """Checks of a matrix that becomes integers; 1 for bfloat16, 0 for float32."""
+    dtype = x.dtype
+    if x.dim() != 2 or not x.is_contiguous() or not x.is_cuda or (dtype is not _BF16 and dtype is not _FP32):
+        check_tensor(name, x)
+        raise KernelError(f"{name} must be a float32 or bfloat16 matrix, got {dtype} {tuple(x.shape)}")
+    if not 0 < x.shape[1] <= MAX_COLUMNS:
+        raise KernelError(f"{name} must have 1 to {MAX_COLUMNS} columns, got {x.shape[1]}")
+    _here(name, x)
+    return 1 if dtype is _BF16 else 0
+
+
+def _here(name: str, x: torch.Tensor) -> None:
+    if x.get_device() != lib._device_index():
+        raise KernelError(f"{name} is on {x.device}, the kernels are launched on cuda:{lib._device_index()}")
+
+
+def _scratch(rows: int, columns: int, device) -> torch.Tensor:
+    return torch.empty(rows * (((columns + 15) & ~15) + 4), dtype=torch.uint8, device=device)
+
+
+def _quantize(x: torch.Tensor, is_bf16: int, delta, norm, rows, eps: float, kind):
+    K = x.shape[1]
     R = rows.numel() if rows is not None else x.shape[0]
-    stride = (K + 15) & ~15
-    values = torch.empty((R, stride), dtype=torch.int8, device=x.device)
-    scales = torch.empty(R, dtype=torch.float32, device=x.device)
-    lib.call("fwb_rows_int8", ptr(x), is_bf16(x), ptr(delta), ptr(norm), ptr(rows), ptr(values), ptr(scales), R, K, stride,
-             eps, stream())
-    return kind(values, scales, K)
-
-
-def _check_rows(name: str, x: torch.Tensor) -> None:
-    check_tensor(name, x)
-    is_bf16(x)
-    if x.dim() != 2 or not 0 < x.shape[1] <= MAX_COLUMNS:
-        raise KernelError(f"{name} must be [rows][1 to {MAX_COLUMNS} columns], got {tuple(x.shape)}")
+    made = kind(_scratch(R, K, x.device), R, K)
+    lib.call("fwb_rows_int8", x.data_ptr(), is_bf16, lib.ptr(delta), lib.ptr(norm), lib.ptr(rows), made._address, made._scales, R, K,
+             made._stride, eps, lib.stream())
+    return made
 
 
 def rows_int8(x: torch.Tensor) -> Int8Rows:
     """Every row of ``x`` ([R][K], bf16 or fp32) as integers of [-127, 127]: ``scale = max|x| / 127`` in fp32,
-    ``value = round(x / scale)``, ties to even.  A row of zeros (nothing above 1e-30) has the scale 0; a row with an infinity
+    ``value = round(x / scale)``, ties to even.  A row of zeros (nothing from 1e-30 on) has the scale 0; a row with an infinity
     or a NaN has the scale NaN."""
-    _check_rows("rows", x)
-    return _quantize(x, None, None, None, 0.0, Int8Rows)
+    return _quantize(x, _input("rows", x), None, None, None, 0.0, Int8Rows)
 
 
 def matrix_int8(w: torch.Tensor) -> Int8Matrix:
     """A weight matrix ([features][K], bf16 or fp32) laid out for the products, once: ``rows_int8`` of its features."""
-    _check_rows("weight", w)
-    made = _quantize(w, None, None, None, 0.0, Int8Matrix)
-    # The products ask for weights before the kernel in front of them has ended.  A launch that is not overlapped with its
+    made = _quantize(w, _input("weight", w), None, None, None, 0.0, Int8Matrix)
+    # The products ask for weights before the kernel in front of them has ended.  A launch that does not overlap its
     # neighbours lies between the two from here on: the copy.
-    made.scales = made.scales.clone()
-    return made
+    return Int8Matrix(made._buffer.clone(), *made.shape)
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optional[torch.Tensor] = None,
@@ -84,33 +110,47 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
     """``ops.rmsnorm`` whose rows leave as integers: ``(x / sqrt(mean(x^2) + eps)) * weight`` per row of the fp32 residual
     ``x``.  With ``delta`` the residual sum ``x += delta`` happens first, in place; with ``rows`` (int32) only those rows are
     normalised, into compact rows (not together with ``delta``)."""
-    check_tensor("residual", x, torch.float32)
-    _check_rows("residual", x)
-    check_tensor("norm weight", weight, torch.float32, (x.shape[1],))
+    if _input("residual", x):
+        raise KernelError("the residual must be float32")
+    check_tensor("norm weight", weight, _FP32, (x.shape[1],))
     if delta is not None:
-        check_tensor("delta", delta, torch.float32, x.shape)
+        check_tensor("delta", delta, _FP32, x.shape)
         if rows is not None:
             raise KernelError("a residual sum goes over every row: delta and rows exclude each other")
     if rows is not None:
         check_tensor("row indices", rows, torch.int32)
-    return _quantize(x, delta, weight, rows, float(eps), Int8Rows)
+    return _quantize(x, 0, delta, weight, rows, float(eps), Int8Rows)
 
 
-def _operands(x, w):
-    if not isinstance(w, Int8Matrix):
+def _product(x: Int8Rows, w: Int8Matrix, out: torch.Tensor, addend, features: int, epilogue: int, limit: float = 0.0,
+             tile: int = 0, splits: int = 1) -> None:
+    lib.call("fwb_gemm_int8", x._address, x._scales, w._address, w._scales, out.data_ptr(), lib.ptr(addend), x._rows, features,
+             x.columns, x._stride, w._stride, w._rows, epilogue, features, limit, tile, splits, lib.stream())
+
+
+def _run(x, w: Int8Matrix, out, out_dtype, addend, features: int, epilogue: int, limit: float) -> torch.Tensor:
+    if type(w) is not Int8Matrix:
         raise KernelError("the weight must be an Int8Matrix (matrix_int8)")
-    if not isinstance(x, Int8Rows):
-        x = rows_int8(x)
-    if x.columns != w.columns:
-        raise KernelError(f"8-bit product: input has {x.columns} columns, weight has {w.columns}")
-    return x
-
-
-def _product(x: Int8Rows, w: Int8Matrix, out: torch.Tensor, addend, features: int, epilogue: int, limit: float = 0.0) -> None:
-    xv, wv = x.values, w.values
-    M = xv.shape[0]
-    lib.call("fwb_gemm_int8", xv.data_ptr(), x.scales.data_ptr(), wv.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             ptr(addend), M, features, x.columns, xv.shape[1], wv.shape[1], wv.shape[0], epilogue, features, limit, stream())
+    ready = isinstance(x, Int8Rows)
+    is_bf16 = 0 if ready else _input("rows", x)
+    M, K = x.shape
+    if K != w.columns:
+        raise KernelError(f"8-bit product: input has {K} columns, weight has {w.columns}")
+    _here("weight", w._buffer)
+    if out is None:
+        out = torch.empty((M, features), dtype=out_dtype, device=w._buffer.device)
+    else:
+        check_tensor("product output", out, out_dtype, (M, features))
+    if addend is not None:
+        check_tensor("product addend", addend, _FP32, (M, features))
+    if ready:
+        _here("rows", x._buffer)
+        _product(x, w, out, addend, features, epilogue, limit)
+    else:
+        scratch = _scratch(M, K, w._buffer.device)
+        lib.call("fwb_linear_int8", x.data_ptr(), is_bf16, scratch.data_ptr(), w._address, w._scales, out.data_ptr(),
+                 lib.ptr(addend), M, features, K, w._stride, w._rows, epilogue, features, limit, lib.stream(), launches=2)
+    return out
 
 
 def linear_int8(x: Union[Int8Rows, torch.Tensor], w: Int8Matrix, out_dtype: torch.dtype,
@@ -118,36 +158,24 @@ def linear_int8(x: Union[Int8Rows, torch.Tensor], w: Int8Matrix, out_dtype: torc
     """``x @ w.T`` [M][N] in fp32 or bf16.  ``x``: integer rows, or a bf16/fp32 matrix, which is brought to integers first.
     ``addend`` (fp32 [M][N], with an fp32 result): added behind the scales; ``out`` may be the addend itself (a residual sum in
     place)."""
-    x = _operands(x, w)
-    shape = (x.values.shape[0], w.values.shape[0])
-    if out_dtype is not torch.float32 and out_dtype is not torch.bfloat16:
+    if out_dtype is _FP32:
+        epilogue = 0 if addend is None else 2
+    elif out_dtype is not _BF16:
         raise KernelError(f"an 8-bit product leaves as float32 or bfloat16, not {out_dtype}")
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=x.values.device)
+    elif addend is not None:
+        raise KernelError("an addend needs a float32 result")
     else:
-        check_tensor("product output", out, out_dtype, shape)
-    epilogue = 1 if out_dtype is torch.bfloat16 else 0
-    if addend is not None:
-        check_tensor("product addend", addend, torch.float32, shape)
-        if epilogue:
-            raise KernelError("an addend needs a float32 result")
-        epilogue = 2
-    _product(x, w, out, addend, shape[1], epilogue)
-    return out
+        epilogue = 1
+    return _run(x, w, out, out_dtype, addend, getattr(w, "_rows", 0), epilogue, 0.0)
 
 
 def gated_int8(x: Union[Int8Rows, torch.Tensor], w: Int8Matrix, activation: str = "silu", limit: float = 0.0) -> torch.Tensor:
     """``act(x @ gate.T) * (x @ up.T)`` as bf16 [M][F], ``w`` holding the F gate rows and then the F up rows; activations as
     ``ops.gate_act_mul``."""
-    from .ops import GATE_ACTIVATIONS
-    x = _operands(x, w)
-    try:
-        act = GATE_ACTIVATIONS[activation]
-    except KeyError:
-        raise KernelError(f"unknown gate activation {activation!r}; known: " + ", ".join(GATE_ACTIVATIONS)) from None
-    rows = w.values.shape[0]
+    act = GATE_ACTIVATIONS.get(activation)
+    if act is None:
+        raise KernelError(f"unknown gate activation {activation!r}; known: " + ", ".join(GATE_ACTIVATIONS))
+    rows = getattr(w, "_rows", 0)
     if rows % 2:
         raise KernelError("gate|up needs an even number of rows")
-    out = torch.empty((x.values.shape[0], rows // 2), dtype=torch.bfloat16, device=x.values.device)
-    _product(x, w, out, None, rows // 2, 3 | act << 8, float(limit))
-    return out
+    return _run(x, w, None, _BF16, None, rows // 2, 3 | act << 8, limit)

@@ -87,6 +87,43 @@ def test_many_values_next_to_a_half():
     assert torch.equal(got.values[:, :x.shape[1]].cpu().to(F64), values)
 
 
+@pytest.mark.parametrize("exponent", [0, -60, 40])
+def test_every_bfloat16_value_under_every_maximum(exponent):
+    """All eight-bit mantissas of ten binades below all eight-bit maxima: the ties of bfloat16 rows are decided without a check."""
+    from flyweight_b200.kernels import int8
+    mantissa = torch.arange(128, 256).to(F64) / 128
+    x = (mantissa[None, :] * 2.0 ** torch.arange(0, -10, -1).to(F64)[:, None]).flatten()
+    rows = torch.cat([mantissa[:, None], x[None, :].expand(128, -1), -x[None, :].expand(128, -1)], dim=1)
+    rows = torch.where(rows.abs() <= mantissa[:, None], rows, torch.zeros_like(rows)) * 2.0 ** exponent
+    stored = rows.to(torch.bfloat16)
+    assert torch.equal(stored.to(F64), rows)
+    values, scale = define(stored)
+    got = int8.rows_int8(stored.to(DEV))
+    assert torch.equal(got.scales.cpu(), scale)
+    assert torch.equal(got.values[:, :rows.shape[1]].cpu().to(F64), values)
+    many = int8.rows_int8(stored.repeat(20, 1).to(DEV))           # the form that many rows take
+    assert torch.equal(many.values[:, :rows.shape[1]].cpu().to(F64), values.repeat(20, 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [24, 300, 520, 1000, 1500, 2048, 3500, 5000, 9000, 16392])
+def test_many_rows_become_the_same_integers_as_few(K, dtype):
+    from flyweight_b200.kernels import int8
+    x = rows_of(2400, K, dtype).to(DEV)
+    many, few = int8.rows_int8(x), int8.rows_int8(x[:100])
+    assert torch.equal(many.values[:100], few.values) and torch.equal(many.scales[:100], few.scales)
+    values, scale = define(x[-50:].cpu())
+    assert torch.equal(many.values[-50:, :K].cpu().to(F64), values) and torch.equal(many.scales[-50:].cpu(), scale)
+    assert not many.values[:, K:].any()
+    if dtype == torch.float32:
+        w = torch.rand(K, device=DEV) + 0.5
+        delta = torch.randn(2400, K, device=DEV)
+        held = x.clone()
+        many, few = int8.rmsnorm_int8(held, w, 1e-5, delta=delta), int8.rmsnorm_int8(x + delta, w, 1e-5)
+        assert torch.equal(held, x + delta)
+        assert torch.equal(many.values, few.values) and torch.equal(many.scales, few.scales)
+
+
 def test_rows_of_zeros_infinities_and_nan():
     from flyweight_b200.kernels import int8
     x = rows_of(6, 200, torch.float32)
@@ -170,6 +207,21 @@ def test_a_row_does_not_depend_on_the_others(M):
     x, matrix = rows_of(600, 1000, torch.bfloat16).to(DEV), int8.matrix_int8(rows_of(700, 1000, torch.bfloat16, 1).to(DEV))
     every, some = int8.linear_int8(x, matrix, torch.float32), int8.linear_int8(x[:M], matrix, torch.float32)
     assert torch.equal(every[:M], some)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 100, 40), (33, 700, 130), (70, 2048, 300), (129, 3000, 257), (300, 130, 600)])
+@pytest.mark.parametrize("tile,splits", [(8, 1), (32, 1), (32, 2), (32, 8), (64, 1), (64, 4), (128, 1), (128, 2), (128, 8), (-128, 1), (-256, 1)])
+def test_every_form_of_the_product_has_the_same_bits(M, K, N, tile, splits):
+    """Forms and cuts that the sizes here would not choose; N is even, so that the same matrix has two halves."""
+    from flyweight_b200.kernels import int8
+    rows, matrix = int8.rows_int8(rows_of(M, K, torch.bfloat16).to(DEV)), int8.matrix_int8(rows_of(2 * N, K, torch.bfloat16, 1).to(DEV))
+    addend = torch.randn(M, 2 * N, generator=torch.Generator().manual_seed(4)).to(DEV)
+    for epilogue, dtype, features in ((0, torch.float32, 2 * N), (1, torch.bfloat16, 2 * N), (2, torch.float32, 2 * N), (3, torch.bfloat16, N)):
+        outs = []
+        for form in ((0, 1), (tile if M <= 32 or tile != 8 else 32, splits)):
+            outs.append(torch.empty((M, features), dtype=dtype, device=DEV))
+            int8._product(rows, matrix, outs[-1], addend if epilogue == 2 else None, features, epilogue, 0.0, *form)
+        assert torch.equal(*outs)
 
 
 def test_the_largest_integers_do_not_overflow():
