@@ -1,0 +1,728 @@
+// Attention of requests that share their first pages, bfloat16, head sizes up to 128, on tensor cores.
+//
+//   prefix kernel   a CTA: 128 rows -- (token, query head of one KV head) pairs of one group -- against one slice of the group's
+//                   shared pages.  As in the prompt kernel (attention_tcgen05.cu): S = Q K^T by tcgen05.mma into one of two
+//                   buffers in tensor memory, a thread a row for the softmax, P back into its scores' columns as bfloat16
+//                   pairs, O += P V with P read from tensor memory.  m follows the running maximum only when that has grown by
+//                   more than 2^8.  Leaves m (in base 2), l and O, not divided, of its slice in scratch, fp32.
+//   own kernel      a CTA: one token, up to 16 query heads of one KV head (the rows of mma.sync 16 x 8 x 16), one slice of the keys behind
+//                   the shared ones; four warps take 16 keys each of every 64-key tile that TMA brings, with a running
+//                   maximum and sum each.  The warps' results meet in shared memory, the slices' in a cluster, the shared
+//                   part's slices from scratch: m = max m_i, O = sum 2^(m_i - m) O_i, l likewise; a sink joins m and l.
+//
+// The shared keys are thus read once for 128 rows.  The own kernel starts as the prefix kernel's CTAs leave and waits for them
+// only ahead of the join: the prefix kernel lets it start when it has itself waited for the kernel in front, so everything that the own
+// kernel reads before the join was written earlier than that.
+//
+// Masked keys are left out by selection; rows of V behind the last key anybody sees are cleared in shared memory, so that
+// 0 * (infinity or NaN) cannot reach a result.  A page id outside the pool is fetched as zeros and masked.
+// Every wait on an mbarrier is bounded: after the limit the CTA raises the library's status word, every role stops waiting, copies
+// in flight land, tensor memory is freed and the CTA returns.
+#include "attention_prefix.cuh"
+#include "tcgen05.cuh"
+
+using namespace fwb;
+using namespace fwb::tc5;
+using namespace fwb::prefix;
+
+namespace {
+
+constexpr int ROWS = 128;        // query rows of a prefix CTA (UMMA M)
+constexpr int KEYS = PAGE;
+constexpr int SOFTMAX_WARPS = 4, PREFIX_THREADS = 64 + 32 * SOFTMAX_WARPS;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int LEAD = 2;                // the scores run this many key tiles ahead of PV
+constexpr float RESCALE_STEP = 8.0f;   // O is rescaled when a row's maximum has grown by more than 2^8
+constexpr int KV_BOX = KEYS * 128;     // 64 keys x 64 channels
+constexpr int OWN_WARPS = 4, OWN_THREADS = 32 * (OWN_WARPS + 1), OWN_ROWS = 16;
+
+struct Params {
+    Batch b;
+    const __nv_bfloat16* q;      // [T][nh * hd]
+    __nv_bfloat16* out;          // [T][nh * hd]
+    float* part_o;               // [T][nh][splits][hd]
+    float* part_ml;              // [T][nh][splits][2]
+    const float* sink;           // [nh] or null
+    int nh, nkv, group, hd, splits, head_chunk, head_chunks;
+    float scale_log2;            // softmax scale * log2(e)
+    float cap_pre, cap_unit;     // capped scores: raw <- cap_unit * tanh(raw * cap_pre), cap_pre = scale / cap,
+                                 // cap_unit = cap / scale, so that the scale that follows gives cap * tanh(score / cap); 0: off
+    int pool_rows;               // num_pages * nkv * 64: a row from here on is fetched as zeros
+    int stages;                  // own kernel: depth of the ring
+    int* status;
+};
+
+template <int HD>
+struct Layout {
+    static constexpr int BOXES = HD / 64;
+    static constexpr int Q_BOX = ROWS * 128, Q_BYTES = BOXES * Q_BOX;
+    static constexpr int KV_BYTES = BOXES * KV_BOX;
+    static constexpr int STAGES = HD == 64 ? 4 : 2;          // ring slots, each one K and one V tile: two CTAs an SM
+    static constexpr int DATA = Q_BYTES + 2 * STAGES * KV_BYTES;
+    static constexpr int SMEM = DATA + 1024 + 256;
+    static constexpr int S_COLS = 2 * KEYS;                  // two S buffers at column 0, O behind them
+    static constexpr int TMEM_COLS = 256;
+};
+
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 2^x on the special-function unit (relative error 2^-22; results below 2^-126 are 0).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// A x B with A (P, bfloat16 pairs in 32-bit columns) read from tensor memory.
+__device__ __forceinline__ void umma_bf16_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// the first row of a page's tile in the pool, seen as rows of hd entries; behind the pool's end for an id that is no page
+__device__ __forceinline__ int tile_row(const Params& prm, int page, int kvh) {
+    return prm.b.is_page(page) ? (page * prm.nkv + kvh) * KEYS : prm.pool_rows;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PREFIX_THREADS, 2)
+prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params prm) {
+    using L = Layout<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_s = base;
+    uint8_t* k_s = q_s + L::Q_BYTES;
+    uint8_t* v_s = k_s + L::STAGES * L::KV_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + L::DATA);
+    uint64_t* empty = full + L::STAGES;
+    uint64_t* q_ready = empty + L::STAGES;
+    uint64_t* s_ready = q_ready + 1;                       // [2]: one per S buffer
+    uint64_t* p_ready = s_ready + 2;                       // [2]: P of a tile is in its S buffer
+    uint64_t* pv_ready = p_ready + 2;                      // [2]
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_ready + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(q_ready, SOFTMAX_WARPS);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&s_ready[b], 1);
+            mbar_init(&p_ready[b], SOFTMAX_WARPS);
+            mbar_init(&pv_ready[b], 1);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();                  // q, the pages and the batch's arrays come from earlier in the stream
+    pdl_launch_dependents();     // (only now: the own kernel goes by everything in front of this one being done)
+
+    // every warp finds the work by itself: the tile's tokens, its slice of the pages, how far anybody sees
+    const int per_tile = ROWS / prm.head_chunk;
+    const TokenTile tile = token_tile(prm.b, blockIdx.x, per_tile);
+    const int pages = tile.count ? prm.b.pages_of(tile.group) : 0, per = pages_per_slice(pages, prm.splits);
+    const int page0 = blockIdx.z * per, page1 = min(pages, page0 + per);
+    if (page0 >= page1) return;                            // (the whole CTA: nobody has allocated or asked for anything)
+    const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
+    const int heads = min(prm.head_chunk, prm.group - head0);
+    const int* table = prm.b.row_of(prm.b.start_of(tile.group));
+    int far = -1;
+    for (int i = lane; i < tile.count; i += 32)
+        if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.positions[tile.first + i]);
+    far = __reduce_max_sync(0xffffffffu, far);
+    int n_tiles = far < 0 || !table ? 0 : min(page1, far / KEYS + 1) - page0;
+    n_tiles = n_tiles < 0 ? 0 : n_tiles;
+
+    if (warp == 1) tmem_alloc(tmem_holder, L::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_holder;
+    int asked = 0;                                         // the producer's: ring slots filled so far
+
+    if (warp == 0) {
+        // Step t brings K tile t and V tile t - LEAD into one ring slot under one barrier: what the MMA issuer needs
+        // next at the same moment.
+        int ids = -1, ids_v = -1;                          // 32 page ids, a lane each: those of K and, a block behind, of V
+        for (int t = 0; n_tiles > 0 && t < n_tiles + LEAD; ++t) {
+            const int s = t % L::STAGES;
+            if (t % 32 == 0) {
+                ids_v = ids;
+                ids = t + lane < n_tiles ? table[page0 + t + lane] : -1;
+            }
+            const int vt = t - LEAD;
+            const int k_page = __shfl_sync(0xffffffffu, ids, t & 31);
+            const int v_page = __shfl_sync(0xffffffffu, t % 32 < LEAD ? ids_v : ids, vt & 31);
+            bool ok = true;
+            if (lane == 0) {
+                if (t >= L::STAGES) ok = mbar_wait(&empty[s], ((t / L::STAGES) - 1) & 1, abort_flag, 51, prm.status);
+                if (ok) {
+                    const bool has_k = t < n_tiles, has_v = vt >= 0;
+                    mbar_expect_tx(&full[s], ((has_k ? 1 : 0) + (has_v ? 1 : 0)) * L::KV_BYTES);
+                    if (has_k) {
+                        const int row = tile_row(prm, k_page, kvh);
+#pragma unroll
+                        for (int b = 0; b < L::BOXES; ++b)
+                            tma_load_2d(k_s + (size_t)s * L::KV_BYTES + b * KV_BOX, &map_k, &full[s], b * 64, row);
+                    }
+                    if (has_v) {
+                        const int row = tile_row(prm, v_page, kvh);
+#pragma unroll
+                        for (int b = 0; b < L::BOXES; ++b)
+                            tma_load_2d(v_s + (size_t)s * L::KV_BYTES + b * KV_BOX, &map_v, &full[s], b * 64, row);
+                    }
+                    ++asked;
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && n_tiles > 0) {
+            constexpr uint32_t idesc_qk = make_idesc_mn(ROWS, KEYS);
+            constexpr uint32_t idesc_pv = make_idesc_mn(ROWS, HD) | IDESC_B_MN_MAJOR;
+            const uint32_t tmem_pv = tmem_base + L::S_COLS, q_addr = smem_u32(q_s);
+            const int k_steps = (prm.hd + UMMA_K - 1) / UMMA_K;
+            // S of tile j goes to buffer j & 1.  One thread issues everything, so a commit also covers every product
+            // issued before it: when S of tile j is ready, PV of tile j - 2 has read its P, which lay in that buffer.
+            bool ok = mbar_wait(q_ready, 0, abort_flag, 52, prm.status);
+            auto wait_step = [&](int u) {
+                const int s = u % L::STAGES;
+                ok = ok && mbar_wait(&full[s], (u / L::STAGES) & 1, abort_flag, 53, prm.status);
+                tc_fence_after();
+                return s;
+            };
+            auto issue_qk = [&](int j, int s) {
+                const uint32_t k_addr = smem_u32(k_s + (size_t)s * L::KV_BYTES);
+                for (int kk = 0; kk < k_steps; ++kk) {
+                    const uint64_t a = make_smem_desc(q_addr + (kk >> 2) * L::Q_BOX) + 2 * (kk & 3);
+                    const uint64_t b = make_smem_desc(k_addr + (kk >> 2) * KV_BOX) + 2 * (kk & 3);
+                    umma_bf16(tmem_base + (j & 1) * KEYS, a, b, idesc_qk, kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_ready[j & 1]);
+            };
+            int u = 0;
+            for (int t = 0; t < LEAD && ok; ++t, ++u) {               // the steps that bring no V yet
+                const int s = wait_step(u);
+                if (!ok) break;
+                if (t < n_tiles) issue_qk(t, s);
+                umma_commit(&empty[s]);
+            }
+            for (int j = 0; j < n_tiles && ok; ++j, ++u) {
+                ok = mbar_wait(&p_ready[j & 1], (j >> 1) & 1, abort_flag, 55, prm.status);
+                const int s = wait_step(u);
+                if (!ok) break;
+                const uint32_t v_addr = smem_u32(v_s + (size_t)s * L::KV_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < KEYS / UMMA_K; ++kk) {
+                    const uint64_t b = make_smem_desc_mn_major(v_addr + kk * 2048, KV_BOX);    // 16 keys: two 8-row groups
+                    umma_bf16_a_tmem(tmem_pv, tmem_base + (j & 1) * KEYS + kk * 8, b, idesc_pv, j > 0 || kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&pv_ready[j & 1]);
+                if (j + LEAD < n_tiles) issue_qk(j + LEAD, s);
+                umma_commit(&empty[s]);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane, swz = row & 7;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + L::S_COLS;
+        const int t_in = row / prm.head_chunk, h_in = row - t_in * prm.head_chunk;
+        const bool valid = t_in < tile.count && h_in < heads;
+        const int tok = tile.first + (valid ? t_in : 0), head = kvh * prm.group + head0 + (valid ? h_in : 0);
+        const int hi = valid && prm.b.row_of(tok) ? prm.b.positions[tok] : -1;
+        bool ok = true;
+        float m = -INFINITY, l = 0.0f;
+        if (n_tiles > 0) {
+            const __nv_bfloat16* q_row = prm.q + ((size_t)tok * prm.nh + head) * prm.hd;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint4 v = valid && c * 8 < prm.hd ? *reinterpret_cast<const uint4*>(q_row + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(q_s + (c >> 3) * L::Q_BOX + row * 128 + (((c & 7) ^ swz) << 4)) = v;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+        }
+        int ids = -1;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int key0 = (page0 + j) * KEYS, buf = j & 1;
+            if (j % 32 == 0) ids = j + lane < n_tiles ? table[page0 + j + lane] : -1;
+            const bool is_page = prm.b.is_page(__shfl_sync(0xffffffffu, ids, j & 31));
+            ok = mbar_wait(&s_ready[buf], (j >> 1) & 1, abort_flag, 56, prm.status);
+            ok = __all_sync(0xffffffffu, ok);              // tcgen05.ld needs the whole warp
+            if (!ok) break;
+            tc_fence_after();
+            float sc[KEYS];
+            tmem_ld64(lane_addr + buf * KEYS, sc);
+            tc_fence_before();
+            if (prm.cap_pre != 0.0f) {
+                // a warp whose scores of this tile all lie far below the cap takes the polynomial: it spares the
+                // special-function unit, which the exponentials need
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    sc[i] *= prm.cap_pre;
+                    top = fmaxf(top, fabsf(sc[i]));
+                }
+                if (__all_sync(0xffffffffu, top <= TANH_SMALL)) {
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) sc[i] = prm.cap_unit * tanh_small_f32(sc[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) sc[i] = prm.cap_unit * tanh_fast_f32(sc[i]);
+                }
+            }
+            // a tile every row sees whole needs no mask (rows without a token are never stored)
+            if (!is_page || !__all_sync(0xffffffffu, !valid || key0 + KEYS - 1 <= hi)) {
+                const int last = is_page ? hi : -1;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) sc[i] = key0 + i <= last ? sc[i] : -INFINITY;
+            }
+            // four interleaved chains each for the maximum and the sum: a fixed order, a quarter of the latency
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[i]);
+            const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * prm.scale_log2;
+            const bool moved = tile_max > m + RESCALE_STEP;          // also: the row's first keys (m = -inf)
+            float factor = 1.0f;
+            if (moved) {
+                factor = ex2(m - tile_max);                          // 2^(-inf) = 0 for the first keys
+                m = tile_max;
+                l *= factor;
+            }
+            if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                // every PV so far has landed in O; scale this warp's rows (by exactly 1 where nothing moved)
+                ok = mbar_wait(&pv_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, 58, prm.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    float v[32];
+                    tmem_ld32(o_addr + c0, v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] *= factor;
+                    tmem_st32(o_addr + c0, v);
+                }
+                tc_fence_before();
+            }
+            const float zero = m == -INFINITY ? 0.0f : m;            // a row that has seen no key yet
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float packed[KEYS / 2];
+#pragma unroll
+            for (int i = 0; i < KEYS; i += 2) {
+                const float p0 = ex2(fmaf(sc[i], prm.scale_log2, -zero));         // masked: 2^(-inf) = 0
+                const float p1 = ex2(fmaf(sc[i + 1], prm.scale_log2, -zero));
+                sum[i & 3] += p0;
+                sum[(i + 1) & 3] += p1;
+                packed[i >> 1] = __uint_as_float(pack2(p0, p1));
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            // P goes back into the columns its scores came from: the buffer's last reader, PV of the tile before the last,
+            // had completed when this tile's S was ready
+            tmem_st32(lane_addr + buf * KEYS, packed);
+            tc_fence_before();
+            const int seen = far + 1 - key0;                          // keys of this tile anybody may see
+            if (seen < KEYS) {
+                // only the last tile: clear the V rows behind it (whole 128-byte rows of every box)
+                const int u = j + LEAD, s = u % L::STAGES;            // the step that brought this V tile
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (u / L::STAGES) & 1, abort_flag, 57, prm.status));
+                uint8_t* v_tile = v_s + (size_t)s * L::KV_BYTES;
+                const int chunks = (KEYS - seen) * 8;
+                for (int b = 0; b < L::BOXES; ++b)
+                    for (int i = threadIdx.x - 64; i < chunks; i += 32 * SOFTMAX_WARPS)
+                        *reinterpret_cast<uint4*>(v_tile + b * KV_BOX + seen * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async();                                  // the cleared rows, for the tensor core
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[buf]);
+        }
+        if (ok && n_tiles > 0) {
+            const int last = n_tiles - 1;
+            ok = mbar_wait(&pv_ready[last & 1], (last >> 1) & 1, abort_flag, 60, prm.status);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (ok) {
+            tc_fence_after();
+            const size_t at = ((size_t)tok * prm.nh + head) * prm.splits + blockIdx.z;
+            // (a slice that a row sees nothing of is left out by its m: its O is not read)
+            if (valid) *reinterpret_cast<float2*>(prm.part_ml + 2 * at) = make_float2(m, l);
+            if (n_tiles > 0) {
+#pragma unroll
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    float v[32];
+                    tmem_ld32(o_addr + c0, v);
+                    if (valid) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            if (c0 + c < prm.hd)
+                                *reinterpret_cast<float4*>(prm.part_o + at * prm.hd + c0 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                    }
+                }
+                tc_fence_before();
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag)
+        for (int s = 0; s < L::STAGES && s < asked; ++s) {           // copies still in flight land first
+            const uint32_t last = (uint32_t)((asked - 1 - s) / L::STAGES) & 1;
+            for (unsigned spin = 0; spin < WAIT_LIMIT && !mbar_test(&full[s], last); ++spin) __nanosleep(64);
+        }
+    if (warp == 1) tmem_dealloc(tmem_base, L::TMEM_COLS);
+}
+
+// ------------------------------------------------------------------ own keys and the join
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// 2^(m - of), 0 for a part that has seen nothing
+__device__ __forceinline__ float part_weight(float m, float of) { return m == -INFINITY ? 0.0f : ex2(m - of); }
+
+template <int HD>
+struct OwnLayout {
+    static constexpr int BOXES = HD / 64, KV_BYTES = BOXES * KV_BOX, STAGE = 2 * KV_BYTES;
+    static constexpr int MERGE_FLOATS = OWN_WARPS * OWN_ROWS * (HD + 2);        // O, m and l of the warps
+    static constexpr int data(int stages) { return stages * STAGE > MERGE_FLOATS * 4 ? stages * STAGE : MERGE_FLOATS * 4; }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(OWN_THREADS, HD == 64 ? 4 : 2)
+own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params prm) {
+    using L = OwnLayout<HD>;
+    constexpr int MAX_STAGES = 8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+    __shared__ int abort_word, page_ok[MAX_STAGES];
+    __shared__ float joined[OWN_ROWS][2];                  // m and l of this CTA's rows, its warps together
+    volatile int* abort_flag = &abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, stages = prm.stages;
+    const int slices = gridDim.z, slice = blockIdx.z;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], OWN_WARPS);
+        }
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_launch_dependents();     // (the kernel behind waits for all of this one)
+    const int t = blockIdx.x, chunks = (prm.group + OWN_ROWS - 1) / OWN_ROWS;
+    const int kvh = blockIdx.y / chunks, head0 = kvh * prm.group + (blockIdx.y % chunks) * OWN_ROWS;
+    const int heads = min(OWN_ROWS, (kvh + 1) * prm.group - head0);
+    const int group = group_of(prm.b, t);
+    if (group < 0) {                                       // rows of no group stay as they are; the whole cluster leaves
+        pdl_wait();
+        return;
+    }
+    const int pages = prm.b.pages_of(group);
+    const int* table = prm.b.row_of(t);
+    const int last = table ? min(prm.b.positions[t], prm.b.max_pages * KEYS - 1) : -1;
+    const int own = last >= pages * KEYS ? last / KEYS + 1 - pages : 0, per = (own + slices - 1) / slices;
+    const int tile0 = pages + slice * per, tile1 = min(pages + own, tile0 + per), n_tiles = max(0, tile1 - tile0);
+    __syncthreads();
+
+    int asked = 0;
+    float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    if (warp == OWN_WARPS) {
+        int ids = -1;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int s = j % stages;
+            if (j % 32 == 0) ids = j + lane < n_tiles ? table[tile0 + j + lane] : -1;
+            const int page = __shfl_sync(0xffffffffu, ids, j & 31);
+            bool ok = true;
+            if (lane == 0) {
+                if (j >= stages) ok = mbar_wait(&empty[s], ((j / stages) - 1) & 1, abort_flag, 61, prm.status);
+                if (ok) {
+                    page_ok[s] = prm.b.is_page(page);
+                    mbar_expect_tx(&full[s], L::STAGE);
+                    const int row = tile_row(prm, page, kvh);
+                    uint8_t* stage = ring + (size_t)s * L::STAGE;
+#pragma unroll
+                    for (int b = 0; b < L::BOXES; ++b) {
+                        tma_load_2d(stage + b * KV_BOX, &map_k, &full[s], b * 64, row);
+                        tma_load_2d(stage + L::KV_BYTES + b * KV_BOX, &map_v, &full[s], b * 64, row);
+                    }
+                    ++asked;
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+        }
+    } else if (n_tiles > 0) {
+        uint32_t qf[HD / 16][4];
+        const __nv_bfloat16* q_at = prm.q + ((size_t)t * prm.nh + head0) * prm.hd;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = g + (i & 1) * 8, c = kk * 16 + (i >> 1) * 8 + t4 * 2;
+                qf[kk][i] = r < heads && c < prm.hd ? *reinterpret_cast<const uint32_t*>(q_at + (size_t)r * prm.hd + c) : 0u;
+            }
+        const int key_k = warp * 16 + (lane >> 4) * 8 + (lane & 7), chunk_k = (lane >> 3) & 1;     // ldmatrix rows of K and V
+        const int key_v = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), chunk_v = lane >> 4;
+        bool ok = true;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int s = j % stages, key0 = (tile0 + j) * KEYS + warp * 16;
+            ok = mbar_wait(&full[s], (j / stages) & 1, abort_flag, 62, prm.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (page_ok[s] && key0 <= last) {
+                const uint32_t k_at = smem_u32(ring + (size_t)s * L::STAGE), v_at = k_at + L::KV_BYTES;
+                float sc[2][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    uint32_t b[4];
+                    const int chunk = (2 * kk + chunk_k) & 7;
+                    ldmatrix_x4(b, k_at + (kk >> 2) * KV_BOX + key_k * 128 + ((chunk ^ (key_k & 7)) << 4));
+                    mma_bf16(sc[0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b[0], b[1]);
+                    mma_bf16(sc[1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b[2], b[3]);
+                }
+                if (prm.cap_pre != 0.0f) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[n][i] = prm.cap_unit * tanh_fast_f32(sc[n][i] * prm.cap_pre);
+                }
+                const bool whole = key0 + 15 <= last;
+                if (!whole) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[n][i] = key0 + n * 8 + t4 * 2 + (i & 1) <= last ? sc[n][i] : -INFINITY;
+                    // the values of keys that nobody sees, whatever they hold (the slice's last tile: nothing is copied over it)
+                    for (int i = lane; i < (15 - (last - key0)) * 8 * L::BOXES; i += 32) {
+                        const int r = warp * 16 + (last - key0) + 1 + (i >> 3) % (15 - (last - key0));
+                        const int box = (i >> 3) / (15 - (last - key0));
+                        *reinterpret_cast<uint4*>(ring + (size_t)s * L::STAGE + L::KV_BYTES + box * KV_BOX + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
+                float factor[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float top = quad_max(fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]))) * prm.scale_log2;
+                    const float now = fmaxf(m[r], top), zero = now == -INFINITY ? 0.0f : now;
+                    factor[r] = ex2(m[r] - zero);
+                    m[r] = now;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 2 * r; i < 2 * r + 2; ++i) {
+                            sc[n][i] = ex2(fmaf(sc[n][i], prm.scale_log2, -zero));
+                            sum += sc[n][i];
+                        }
+                    l[r] = l[r] * factor[r] + sum;
+                }
+                const uint32_t p0 = pack2(sc[0][0], sc[0][1]), p1 = pack2(sc[0][2], sc[0][3]), p2 = pack2(sc[1][0], sc[1][1]), p3 = pack2(sc[1][2], sc[1][3]);
+                if (__any_sync(0xffffffffu, factor[0] != 1.0f || factor[1] != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i) o[i][0] *= factor[0], o[i][1] *= factor[0], o[i][2] *= factor[1], o[i][3] *= factor[1];
+                }
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {
+                    uint32_t b[4];
+                    const int chunk = (n + chunk_v) & 7;
+                    ldmatrix_x4_trans(b, v_at + (n >> 3) * KV_BOX + key_v * 128 + ((chunk ^ (key_v & 7)) << 4));
+                    mma_bf16(o[n], p0, p1, p2, p3, b[0], b[1]);
+                    mma_bf16(o[n + 1], p0, p1, p2, p3, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        if (warp == OWN_WARPS && lane == 0)
+            for (int s = 0; s < stages && s < asked; ++s) {          // copies still in flight land first
+                const uint32_t done = (uint32_t)((asked - 1 - s) / stages) & 1;
+                for (unsigned spin = 0; spin < WAIT_LIMIT && !mbar_test(&full[s], done); ++spin) __nanosleep(64);
+            }
+        __syncthreads();
+    }
+    // the warps' parts into shared memory, where the ring was: o_s [warp][row][HD], ml_s [warp][row][2]
+    float* o_s = reinterpret_cast<float*>(ring);
+    float* ml_s = o_s + OWN_WARPS * OWN_ROWS * HD;
+    if (warp < OWN_WARPS) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] = quad_sum(l[r]);
+            const int row = warp * OWN_ROWS + g + 8 * r;
+            if (t4 == 0) ml_s[2 * row] = m[r], ml_s[2 * row + 1] = l[r];
+            if (g + 8 * r < heads) {
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n)
+                    *reinterpret_cast<float2*>(o_s + row * HD + n * 8 + t4 * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+            }
+        }
+    }
+    __syncthreads();
+    // this CTA's warps together (rows stay in o_s's first quarter): every thread has channels of rows
+    if (threadIdx.x < OWN_ROWS) {
+        const int row = threadIdx.x;
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < OWN_WARPS; ++w) top = fmaxf(top, ml_s[2 * (w * OWN_ROWS + row)]);
+        for (int w = 0; w < OWN_WARPS; ++w) {
+            const float f = part_weight(ml_s[2 * (w * OWN_ROWS + row)], top);
+            sum += f * ml_s[2 * (w * OWN_ROWS + row) + 1];
+            ml_s[2 * (w * OWN_ROWS + row)] = f;            // from here on: the warp's weight
+        }
+        joined[row][0] = top, joined[row][1] = sum;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * HD; i += OWN_THREADS) {
+        const int row = i / HD;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < OWN_WARPS; ++w) {
+            const float f = ml_s[2 * (w * OWN_ROWS + row)];
+            if (f != 0.0f) v = fmaf(f, o_s[(w * OWN_ROWS) * HD + i], v);
+        }
+        o_s[i] = v;
+    }
+    pdl_wait();                  // the shared part is there
+    const bool cluster = slices > 1;
+    if (cluster) cluster_sync_all();
+    else __syncthreads();
+    // the join: with a cluster every CTA has a share of the rows
+    const int shared_per = pages_per_slice(pages, prm.splits), shared = shared_per ? (pages + shared_per - 1) / shared_per : 0;
+    const uint32_t o_at = smem_u32(o_s), ml_at = smem_u32(joined);
+    constexpr int LANES = HD / 4;                          // threads a row, four channels each
+    for (int i = threadIdx.x; i < heads * LANES; i += OWN_THREADS) {
+        const int row = i / LANES, c = (i - row * LANES) * 4, head = head0 + row;
+        if (cluster && row % slices != slice) continue;
+        const size_t at = ((size_t)t * prm.nh + head) * prm.splits;
+        const float sink = prm.sink ? prm.sink[head] * LOG2E : -INFINITY;
+        float top = sink;
+        for (int s = 0; s < slices; ++s) top = fmaxf(top, cluster ? ld_dsmem_f32(ml_at + row * 8, s) : joined[row][0]);
+        for (int s = 0; s < shared; ++s) top = fmaxf(top, prm.part_ml[2 * (at + s)]);
+        float sum = part_weight(sink, top);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto add = [&](float f, const float4& x) {
+            v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+        };
+        for (int s = 0; s < slices; ++s) {
+            const float f = part_weight(cluster ? ld_dsmem_f32(ml_at + row * 8, s) : joined[row][0], top);
+            if (f == 0.0f) continue;
+            sum = fmaf(f, cluster ? ld_dsmem_f32(ml_at + row * 8 + 4, s) : joined[row][1], sum);
+            add(f, cluster ? ld_dsmem_f32x4(o_at + (uint32_t)(row * HD + c) * 4, s) : *reinterpret_cast<const float4*>(o_s + row * HD + c));
+        }
+        if (c < prm.hd)
+            for (int s = 0; s < shared; ++s) {
+                const float2 ml = *reinterpret_cast<const float2*>(prm.part_ml + 2 * (at + s));
+                const float f = part_weight(ml.x, top);
+                if (f == 0.0f) continue;
+                sum = fmaf(f, ml.y, sum);
+                add(f, *reinterpret_cast<const float4*>(prm.part_o + (at + s) * prm.hd + c));
+            }
+        if (c < prm.hd && !*abort_flag) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<uint2*>(prm.out + ((size_t)t * prm.nh + head) * prm.hd + c) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+        }
+    }
+    if (cluster) cluster_sync_all();                       // nobody leaves while a peer still reads from it
+}
+
+template <int HD>
+int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int own_slices, cudaStream_t stream) {
+    using L = Layout<HD>;
+    auto prefix = prefix_tcgen05_kernel<HD>;
+    auto own = own_kernel<HD>;
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(prefix, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    const long tiles = most_token_tiles(prm.b.T, prm.b.n_groups, ROWS / prm.head_chunk);
+    fwb::pdl(prefix, dim3((unsigned)tiles, prm.nkv * prm.head_chunks, prm.splits), PREFIX_THREADS, L::SMEM, stream)(map_k, map_v, prm);
+    int e = fwb_launch_status();
+    if (e) return e;
+    prm.stages = HD == 64 ? 3 : 2;
+    const int chunks = (prm.group + OWN_ROWS - 1) / OWN_ROWS;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(prm.b.T, prm.nkv * chunks, own_slices);
+    config.blockDim = dim3(OWN_THREADS);
+    config.dynamicSmemBytes = OwnLayout<HD>::data(prm.stages) + 1024;
+    config.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (own_slices > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = own_slices;
+    }
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    config.attrs = attr;
+    config.numAttrs = n;
+    cudaError_t status = cudaLaunchKernelEx(&config, own, map_k, map_v, prm);
+    return status == cudaSuccess ? fwb_launch_status() : (int)status;
+}
+
+}  // namespace
+
+namespace fwb {
+namespace prefix {
+
+bool tensor_cores_take(const void* q, const void* k_pool, const void* v_pool, const void* out, const void* part_o, const Batch& b, int nkv, int hd) {
+    return hd % 8 == 0 && hd <= 128 && (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)part_o) & 15) == 0 &&
+           (long)b.num_pages * nkv * PAGE <= 2147483647L - PAGE;
+}
+
+int launch_tensor_cores(const Batch& b, const void* q, const void* k_pool, const void* v_pool, void* out, float* part_o, float* part_ml,
+                        const float* sink, int nh, int nkv, int hd, int splits, int own_slices, float scale, float softcap,
+                        cudaStream_t stream) {
+    Params prm{};
+    prm.b = b;
+    prm.q = static_cast<const __nv_bfloat16*>(q);
+    prm.out = static_cast<__nv_bfloat16*>(out);
+    prm.part_o = part_o, prm.part_ml = part_ml, prm.sink = sink;
+    prm.nh = nh, prm.nkv = nkv, prm.group = nh / nkv, prm.hd = hd, prm.splits = splits;
+    prm.head_chunk = prm.group < ROWS ? prm.group : ROWS;
+    prm.head_chunks = (prm.group + prm.head_chunk - 1) / prm.head_chunk;
+    prm.scale_log2 = scale * LOG2E;
+    prm.cap_pre = softcap > 0.0f ? scale / softcap : 0.0f;
+    prm.cap_unit = softcap > 0.0f ? softcap / scale : 0.0f;
+    const long rows = (long)b.num_pages * nkv * PAGE;
+    prm.pool_rows = (int)rows;
+    prm.status = status_word();
+    CUtensorMap map_k, map_v;
+    if (!make_map(&map_k, k_pool, rows, hd, KEYS) || !make_map(&map_v, v_pool, rows, hd, KEYS)) return FWB_UNSUPPORTED;
+    return hd <= 64 ? launch<64>(map_k, map_v, prm, own_slices, stream) : launch<128>(map_k, map_v, prm, own_slices, stream);
+}
+
+}  // namespace prefix
+}  // namespace fwb

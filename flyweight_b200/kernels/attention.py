@@ -266,10 +266,15 @@ def paged_attention(ctx, q, cache, block_table, n_heads, window, scale, out_dtyp
                               keep_first=keep_first)
 
 
-def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int) -> int:
-    """How many slices of a group's shared pages run as separate blocks."""
-    row_tiles = max(1, -(-n_tokens * group // 64)) * n_kv
-    return max(1, min(shared_pages, 64, -(-2 * SM_COUNT // row_tiles)))
+def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int, own_pages: int, wide: bool):
+    """How the work of ``shared_prefix_attention`` is cut: slices of a group's shared pages, slices of a token's own ones.
+    ``wide``: 128 rows a block and two blocks an SM (the tensor cores), else 64 and one or two."""
+    row_tiles = -(-n_tokens * group // (128 if wide else 64)) * n_kv
+    shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles))
+    own, pairs = 1, n_tokens * n_kv * -(-group // 16)
+    while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and own_pages >= 8 * own:
+        own *= 2
+    return shared, own
 
 
 def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, group_start, group_pages, n_heads: int,
@@ -323,10 +328,12 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     if T == 0 or groups == 0:
         return out
     width = block_table.shape[1]
-    splits = shared_prefix_splits(T, n_kv, n_heads // n_kv, min(width, width if shared_pages is None else max(1, shared_pages)))
+    wide = q.dtype == torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
+    splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, width if shared_pages is None else min(width, shared_pages),
+                                       width if own_pages is None else own_pages, wide)
     part_o = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
     part_ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
     lib.call("fwb_attention_prefix", ptr(q), ptr(k_pool), ptr(v_pool), is_bf16(q), ptr(positions), ptr(tok_seg), ptr(block_table),
              block_table.shape[0], width, num_pages, ptr(group_start), ptr(group_pages), groups, ptr(part_o), ptr(part_ml),
-             ptr(out), T, n_heads, n_kv, head_dim, splits, c_float(scale), ptr(sink), c_float(softcap), stream(), launches=2)
+             ptr(out), T, n_heads, n_kv, head_dim, splits, own, c_float(scale), ptr(sink), c_float(softcap), stream(), launches=2)
     return out
