@@ -28,6 +28,7 @@ struct Params {
     void* out;                   // [T][nh * hd]
     const float* sink;           // [nh] or null
     int nh, nkv, group, hd, splits, head_chunk, head_chunks;
+    int vector;                  // rows of four channels start on borders of four elements
     float scale, cap;
 };
 
@@ -36,13 +37,33 @@ __device__ __forceinline__ float score(const Params& prm, float dot) {
     return prm.cap > 0.0f ? prm.cap * tanhf(s / prm.cap) : s;
 }
 
-// a page's tile of one KV head into shared memory, rows `pitch` floats apart; rows from `rows` on become zero
+__device__ __forceinline__ float4 load4(const float* at) { return *reinterpret_cast<const float4*>(at); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* at) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+// A page's tiles of one KV head, keys and values, into shared memory: rows `pitch` and `v_pitch` floats apart, channels from hd
+// up to the next multiple of four and rows from `rows` on zero.
 template <typename T>
-__device__ __forceinline__ void load_tile(float* to, const void* pool, size_t tile, int rows, int hd, int pitch) {
-    const T* from = reinterpret_cast<const T*>(pool) + tile * PAGE * hd;
-    for (int i = threadIdx.x; i < PAGE * hd; i += THREADS) {
-        const int r = i / hd, c = i - r * hd;
-        to[r * pitch + c] = r < rows ? to_f32(from[i]) : 0.0f;
+__device__ __forceinline__ void load_tiles(const Params& prm, float* k_s, int pitch, float* v_s, int v_pitch, size_t tile, int rows) {
+    const int hd = prm.hd, quads = (hd + 3) >> 2;
+    const T *k = reinterpret_cast<const T*>(prm.k) + tile * PAGE * hd, *v = reinterpret_cast<const T*>(prm.v) + tile * PAGE * hd;
+    const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (prm.vector) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < PAGE * quads; i += THREADS) {
+            const int r = i / quads, c = (i - r * quads) * 4;
+            const float4 a = r < rows ? load4(k + i * 4) : none, b = r < rows ? load4(v + i * 4) : none;
+            *reinterpret_cast<float4*>(k_s + r * pitch + c) = a;
+            *reinterpret_cast<float4*>(v_s + r * v_pitch + c) = b;
+        }
+    } else {
+        for (int i = threadIdx.x; i < PAGE * quads * 4; i += THREADS) {
+            const int r = i / (quads * 4), c = i - r * quads * 4;
+            const bool live = r < rows && c < hd;
+            k_s[r * pitch + c] = live ? to_f32(k[r * hd + c]) : 0.0f;
+            v_s[r * v_pitch + c] = live ? to_f32(v[r * hd + c]) : 0.0f;
+        }
     }
 }
 
@@ -59,12 +80,12 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
     const int per_tile = ROWS / prm.head_chunk;
     const TokenTile tile = token_tile(prm.b, blockIdx.x, per_tile);
     if (tile.count == 0) return;
-    const int pages = prm.b.pages_of(tile.group), per = pages_per_slice(pages, prm.splits);
+    const int pages = tile.pages, per = pages_per_slice(pages, prm.splits);
     const int page0 = blockIdx.z * per, page1 = min(pages, page0 + per);
     if (page0 >= page1) return;
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
-    const int* table = prm.b.row_of(prm.b.start_of(tile.group));
+    const int* table = prm.b.row_of(tile.group_first);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 
     for (int i = threadIdx.x; i < ROWS * pitch; i += THREADS) {
@@ -92,11 +113,10 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
         const int page = table ? table[p] : -1;
         if (!prm.b.is_page(page)) continue;            // (nothing is read where no page is)
         __syncthreads();
-        load_tile<T>(k_s, prm.k, (size_t)page * prm.nkv + kvh, PAGE, hd, pitch);
-        load_tile<T>(v_s, prm.v, (size_t)page * prm.nkv + kvh, PAGE, hd, COLS * 64);
+        load_tiles<T>(prm, k_s, pitch, v_s, COLS * 64, (size_t)page * prm.nkv + kvh, PAGE);
         __syncthreads();
         float s[4][4] = {};
-        for (int d = 0; d + 3 < hd; d += 4) {
+        for (int d = 0; d < hd; d += 4) {               // (channels behind the last are zero in both)
             float4 a[4], b[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ty * 4 + i) * pitch + d);
@@ -108,11 +128,6 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
                 for (int j = 0; j < 4; ++j)
                     s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
         }
-        for (int d = hd & ~3; d < hd; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] = fmaf(q_s[(ty * 4 + i) * pitch + d], k_s[(tx + 16 * j) * pitch + d], s[i][j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = -INFINITY;
@@ -177,47 +192,61 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
     }
 }
 
+// (threads as (part of the keys, head, four channels) for O: items of head and channels, `parts` threads an item)
 template <typename T>
 __global__ void __launch_bounds__(THREADS) own_kernel(const Params prm) {
     extern __shared__ float smem[];
-    const int hd = prm.hd, pitch = ((hd + 3) & ~3) + 4;
+    const int hd = prm.hd, quads = (hd + 3) >> 2, pitch = quads * 4 + 4;
     float* q_s = smem;                                 // [OWN_HEADS][pitch]
     float* k_s = q_s + OWN_HEADS * pitch;              // [PAGE][pitch]
-    float* v_s = k_s + PAGE * pitch;                   // [PAGE][hd]
-    float* p_s = v_s + PAGE * hd;                      // [OWN_HEADS][PAGE]
+    float* v_s = k_s + PAGE * pitch;                   // [PAGE][quads * 4]
+    float* p_s = v_s + PAGE * quads * 4;               // [OWN_HEADS][PAGE]
     float* m_s = p_s + OWN_HEADS * PAGE;               // [OWN_HEADS], and the two behind it
     float* l_s = m_s + OWN_HEADS;
     float* f_s = l_s + OWN_HEADS;
-    pdl_wait();
+    __shared__ float shared_weight[OWN_HEADS][MAX_SPLITS], own_weight[OWN_HEADS], inverse[OWN_HEADS];
+    // (the prefix kernel has waited for what lies in front of it before it let this one start: only its own results are missing)
     pdl_launch_dependents();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunks = (prm.group + OWN_HEADS - 1) / OWN_HEADS;
     const int kvh = blockIdx.y / chunks, head0 = kvh * prm.group + (blockIdx.y % chunks) * OWN_HEADS;
     const int heads = min(OWN_HEADS, (kvh + 1) * prm.group - head0);
-    const int group = group_of(prm.b, t);
-    if (group < 0) return;                             // rows of no group stay as they are
-    const int pages = prm.b.pages_of(group);
-    const int* table = prm.b.row_of(t);
-    const int last = table ? min(prm.b.positions[t], prm.b.max_pages * PAGE - 1) : -1;
-    for (int i = threadIdx.x; i < OWN_HEADS * pitch; i += THREADS) {
+    const Token token = token_of(prm.b, t);
+    if (token.pages < 0) {                             // rows of no group stay as they are
+        pdl_wait();
+        return;
+    }
+    const int pages = token.pages, last = token.last;
+    for (int i = threadIdx.x; i < heads * pitch; i += THREADS) {
         const int h = i / pitch, c = i - h * pitch;
-        q_s[i] = h < heads && c < hd ? to_f32(reinterpret_cast<const T*>(prm.q)[((size_t)t * prm.nh + head0 + h) * hd + c]) : 0.0f;
+        q_s[i] = c < hd ? to_f32(reinterpret_cast<const T*>(prm.q)[((size_t)t * prm.nh + head0 + h) * hd + c]) : 0.0f;
     }
     if (threadIdx.x < OWN_HEADS) m_s[threadIdx.x] = -INFINITY, l_s[threadIdx.x] = 0.0f;
-    float acc[OWN_HEADS] = {};                         // column threadIdx.x of every head (head sizes up to 256)
-    const int c = threadIdx.x;
+    const int items = heads * quads, parts = items >= THREADS ? 1 : THREADS / items < PAGE ? THREADS / items : PAGE;
+    constexpr int MOST = OWN_HEADS * 64 / THREADS;     // items a thread has at most (head sizes up to 256)
+    float4 acc[MOST];
+#pragma unroll
+    for (int n = 0; n < MOST; ++n) acc[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int part = parts > 1 ? threadIdx.x / items : 0, item0 = parts > 1 ? threadIdx.x - part * items : threadIdx.x;
+    const bool works = part < parts;
     for (int p = pages; p * PAGE <= last; ++p) {
-        const int page = table[p], seen = min(PAGE, last + 1 - p * PAGE);
+        const int page = token.table[p], seen = min(PAGE, last + 1 - p * PAGE);
         if (!prm.b.is_page(page)) continue;
         __syncthreads();
-        load_tile<T>(k_s, prm.k, (size_t)page * prm.nkv + kvh, seen, hd, pitch);
-        load_tile<T>(v_s, prm.v, (size_t)page * prm.nkv + kvh, seen, hd, hd);
+        load_tiles<T>(prm, k_s, pitch, v_s, quads * 4, (size_t)page * prm.nkv + kvh, seen);
         __syncthreads();
-        for (int i = threadIdx.x; i < OWN_HEADS * PAGE; i += THREADS) {
-            const int h = i / PAGE, key = i % PAGE;
-            float dot = 0.0f;
-            for (int d = 0; d < hd; ++d) dot = fmaf(q_s[h * pitch + d], k_s[key * pitch + d], dot);
-            p_s[i] = h < heads && key < seen ? score(prm, dot) : -INFINITY;
+        {
+            const int key = threadIdx.x & 63;
+            for (int h = threadIdx.x >> 6; h < heads; h += THREADS / 64) {
+                float d0 = 0.0f, d1 = 0.0f;
+#pragma unroll 4
+                for (int d = 0; d < quads; ++d) {
+                    const float4 a = *reinterpret_cast<const float4*>(q_s + h * pitch + 4 * d), b = *reinterpret_cast<const float4*>(k_s + key * pitch + 4 * d);
+                    d0 = fmaf(a.x, b.x, fmaf(a.y, b.y, d0));
+                    d1 = fmaf(a.z, b.z, fmaf(a.w, b.w, d1));
+                }
+                p_s[h * PAGE + key] = key < seen ? score(prm, d0 + d1) : -INFINITY;
+            }
         }
         __syncthreads();
         for (int h = warp; h < heads; h += THREADS / 32) {
@@ -233,33 +262,73 @@ __global__ void __launch_bounds__(THREADS) own_kernel(const Params prm) {
             }
         }
         __syncthreads();
-        if (c < hd) {
 #pragma unroll
-            for (int h = 0; h < OWN_HEADS; ++h) {
-                if (h >= heads) break;
-                float a = acc[h] * f_s[h];
-                for (int key = 0; key < seen; ++key) a = fmaf(p_s[h * PAGE + key], v_s[key * hd + c], a);
-                acc[h] = a;
+        for (int n = 0; n < MOST; ++n) {
+            const int item = item0 + n * THREADS, h = item / quads, c = (item - h * quads) * 4;
+            if (!works || item >= items) break;
+            const float f = f_s[h];
+            float4 a = acc[n];
+            a.x *= f, a.y *= f, a.z *= f, a.w *= f;
+            for (int key = part; key < seen; key += parts) {
+                const float w = p_s[h * PAGE + key];
+                const float4 x = *reinterpret_cast<const float4*>(v_s + key * quads * 4 + c);
+                a.x = fmaf(w, x.x, a.x), a.y = fmaf(w, x.y, a.y), a.z = fmaf(w, x.z, a.z), a.w = fmaf(w, x.w, a.w);
             }
+            acc[n] = a;
         }
     }
+    pdl_wait();                                        // the shared part is there
     __syncthreads();
-    const int per = pages_per_slice(pages, prm.splits), slices = per ? (pages + per - 1) / per : 0;
+    // the parts' sums where K was; the weights of the slices, a warp a head and a lane a slice
+    float4* sums = reinterpret_cast<float4*>(k_s);     // [parts][items]
 #pragma unroll
-    for (int h = 0; h < OWN_HEADS; ++h) {
-        if (h >= heads || c >= hd) break;
+    for (int n = 0; n < MOST; ++n)
+        if (works && item0 + n * THREADS < items) sums[part * items + item0 + n * THREADS] = acc[n];
+    const int per = pages_per_slice(pages, prm.splits), slices = per ? (pages + per - 1) / per : 0;
+    for (int h = warp; h < heads; h += THREADS / 32) {
         const size_t at = ((size_t)t * prm.nh + head0 + h) * prm.splits;
-        float top = fmaxf(m_s[h], prm.sink ? prm.sink[head0 + h] : -INFINITY);
-        for (int s = 0; s < slices; ++s) top = fmaxf(top, prm.part_ml[2 * (at + s)]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float factor = expf(m_s[h] - base), o = acc[h] * factor, l = l_s[h] * factor;
-        if (prm.sink) l += expf(prm.sink[head0 + h] - base);
-        for (int s = 0; s < slices; ++s) {
-            factor = expf(prm.part_ml[2 * (at + s)] - base);
-            o = fmaf(factor, prm.part_o[(at + s) * hd + c], o);
-            l = fmaf(factor, prm.part_ml[2 * (at + s) + 1], l);
+        const float sink = prm.sink ? prm.sink[head0 + h] : -INFINITY;
+        float2 of[(MAX_SPLITS + 31) / 32];
+        float top = fmaxf(m_s[h], sink);
+#pragma unroll
+        for (int i = 0; i < (MAX_SPLITS + 31) / 32; ++i) {
+            of[i] = lane + 32 * i < slices ? *reinterpret_cast<const float2*>(prm.part_ml + 2 * (at + lane + 32 * i)) : make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, of[i].x);
         }
-        reinterpret_cast<T*>(prm.out)[((size_t)t * prm.nh + head0 + h) * hd + c] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
+        top = warp_max(top);
+        const float base = top == -INFINITY ? 0.0f : top, mine = expf(m_s[h] - base);
+        float sum = lane == 0 ? l_s[h] * mine + expf(sink - base) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < (MAX_SPLITS + 31) / 32; ++i) {
+            const float w = expf(of[i].x - base);
+            if (lane + 32 * i < slices) shared_weight[h][lane + 32 * i] = w;
+            sum = fmaf(w, of[i].y, sum);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) own_weight[h] = mine, inverse[h] = sum;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += THREADS) {
+        const int h = i / quads, c = (i - h * quads) * 4;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < parts; ++n) {
+            const float4 x = sums[n * items + i];
+            o[0] += x.x, o[1] += x.y, o[2] += x.z, o[3] += x.w;
+        }
+        const float* from = prm.part_o + ((size_t)t * prm.nh + head0 + h) * prm.splits * hd + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j >= hd) break;
+            o[j] *= own_weight[h];
+            // (a slice that weighs nothing may hold anything: it is not read)
+#pragma unroll 4
+            for (int s = 0; s < slices; ++s) {
+                const float w = shared_weight[h][s];
+                o[j] = fmaf(w, w != 0.0f ? from[(size_t)s * hd + j] : 0.0f, o[j]);
+            }
+            const float total = inverse[h];
+            reinterpret_cast<T*>(prm.out)[((size_t)t * prm.nh + head0 + h) * hd + c + j] = from_f32<T>(total == 0.0f ? 0.0f : o[j] / total);
+        }
     }
 }
 
@@ -285,7 +354,7 @@ int launch(const Params& prm, cudaStream_t stream) {
             : launch_prefix<T, 4>(prm, stream);
     if (e) return e;
     const int pitch = ((prm.hd + 3) & ~3) + 4, chunks = (prm.group + OWN_HEADS - 1) / OWN_HEADS;
-    const size_t smem = (size_t)(OWN_HEADS * pitch + PAGE * pitch + PAGE * prm.hd + OWN_HEADS * PAGE + 3 * OWN_HEADS) * 4;
+    const size_t smem = (size_t)(OWN_HEADS * pitch + PAGE * pitch + PAGE * (pitch - 4) + OWN_HEADS * PAGE + 3 * OWN_HEADS) * 4;
     e = configure(own_kernel<T>, smem);
     if (e) return e;
     fwb::pdl(own_kernel<T>, dim3(prm.b.T, prm.nkv * chunks), THREADS, smem, stream)(prm);
@@ -309,7 +378,7 @@ FWB_API int fwb_attention_prefix(const void* q, const void* k_pool, const void* 
         (own_slices != 1 && own_slices != 2 && own_slices != 4 && own_slices != 8))
         return FWB_BAD_ARGUMENT;
     if (nkv <= 0 || nh <= 0 || nh % nkv || hd < 1 || hd > 256) return FWB_UNSUPPORTED;
-    if (nkv > 4095 || max_pages > 33554431 || splits > 65535) return FWB_TOO_LARGE;
+    if (nkv > 4095 || max_pages > 33554431 || splits > MAX_SPLITS) return FWB_TOO_LARGE;
     if (softcap > 0.0f && scale == 0.0f) return FWB_UNSUPPORTED;
     Params prm{};
     prm.b = Batch{positions, tok_seg, block_table, group_start, group_pages, T, n_segments, n_groups, max_pages, num_pages};
@@ -319,6 +388,7 @@ FWB_API int fwb_attention_prefix(const void* q, const void* k_pool, const void* 
     prm.nh = nh, prm.nkv = nkv, prm.group = nh / nkv, prm.hd = hd, prm.splits = splits;
     prm.head_chunk = prm.group < ROWS ? prm.group : ROWS;
     prm.head_chunks = (prm.group + prm.head_chunk - 1) / prm.head_chunk;
+    prm.vector = hd % 4 == 0 && (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0;
     prm.scale = scale, prm.cap = softcap;
     return is_bf16 ? launch<__nv_bfloat16>(prm, stream) : launch<float>(prm, stream);
 }

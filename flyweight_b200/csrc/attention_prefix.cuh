@@ -11,6 +11,7 @@ namespace fwb {
 namespace prefix {
 
 constexpr int PAGE = 64;
+constexpr int MAX_SPLITS = 64;           // slices of a group's shared pages
 
 struct Batch {
     const int* positions;        // [T]
@@ -36,16 +37,16 @@ struct Batch {
     __device__ __forceinline__ bool is_page(int page) const { return page >= 0 && page < num_pages; }
 };
 
-// The token tile `index` when every group's tokens are cut into tiles of `per_tile`: its group, first token and tokens (0: no
-// such tile).  Asked by whole warps.
+// The token tile `index` when every group's tokens are cut into tiles of `per_tile`: its group's first token and pages, its own
+// first token and tokens (0: no such tile).  Asked by whole warps; everything it reads is asked for at once.
 struct TokenTile {
-    int group, first, count;
+    int group_first, pages, first, count;
 };
 __device__ __forceinline__ TokenTile token_tile(const Batch& b, int index, int per_tile) {
     const int lane = threadIdx.x & 31;
     for (int g0 = 0; g0 < b.n_groups; g0 += 32) {
         const int g = g0 + lane;
-        const int first = g < b.n_groups ? b.start_of(g) : 0;
+        const int first = g < b.n_groups ? b.start_of(g) : 0, pages = g < b.n_groups ? b.pages_of(g) : 0;
         int n = g < b.n_groups ? b.start_of(g + 1) - first : 0;
         n = n < 0 ? 0 : n;
         const int tiles = (n + per_tile - 1) / per_tile;
@@ -60,15 +61,16 @@ __device__ __forceinline__ TokenTile token_tile(const Batch& b, int index, int p
             const int owner = __ffs(behind) - 1;
             const int inside = index - (__shfl_sync(0xffffffffu, upto, owner) - __shfl_sync(0xffffffffu, tiles, owner));
             TokenTile t;
-            t.group = g0 + owner;
-            t.first = __shfl_sync(0xffffffffu, first, owner) + inside * per_tile;
+            t.group_first = __shfl_sync(0xffffffffu, first, owner);
+            t.pages = __shfl_sync(0xffffffffu, pages, owner);
+            t.first = t.group_first + inside * per_tile;
             const int left = __shfl_sync(0xffffffffu, n, owner) - inside * per_tile;
             t.count = left < per_tile ? left : per_tile;
             return t;
         }
         index -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    return TokenTile{0, 0, 0};
+    return TokenTile{0, 0, 0, 0};
 }
 // The most such tiles a batch can have, from what the host knows.
 inline long most_token_tiles(int T, int n_groups, int per_tile) {
@@ -76,13 +78,29 @@ inline long most_token_tiles(int T, int n_groups, int per_tile) {
     return most < T ? most : T;
 }
 
-// The group of a token, -1 for one behind the last group (or in front of the first).  Asked by whole warps.
-__device__ __forceinline__ int group_of(const Batch& b, int token) {
+// A token as the own kernels see it: its group's shared pages (-1: it is in no group), its block-table row and the last key it
+// sees.  Asked by whole warps; the group's arrays and the token's are asked for at once.
+struct Token {
+    int pages, last;
+    const int* table;
+};
+__device__ __forceinline__ Token token_of(const Batch& b, int token) {
     const int lane = threadIdx.x & 31;
-    int begun = 0;                                     // groups that start at or before the token
-    for (int g0 = 0; g0 <= b.n_groups; g0 += 32)
-        begun += __popc(__ballot_sync(0xffffffffu, g0 + lane <= b.n_groups && b.start_of(g0 + lane) <= token));
-    return begun > b.n_groups ? -1 : begun - 1;
+    const int seg = b.tok_seg[token], position = b.positions[token];
+    Token t{-1, -1, nullptr};
+    for (int g0 = 0; g0 <= b.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        const bool begun = g <= b.n_groups && b.start_of(g) <= token;
+        const int pages = g < b.n_groups ? b.pages_of(g) : -1;       // (behind the last group: in none)
+        const int n = __popc(__ballot_sync(0xffffffffu, begun));
+        if (n > 0) t.pages = __shfl_sync(0xffffffffu, pages, n - 1);
+        if (n < 32) break;
+    }
+    if (seg >= 0 && seg < b.n_segments) {
+        t.table = b.block_table + (size_t)seg * b.max_pages;
+        t.last = position < b.max_pages * PAGE ? position : b.max_pages * PAGE - 1;
+    }
+    return t;
 }
 
 // How a group's shared pages are cut into at most `splits` slices: pages a slice.

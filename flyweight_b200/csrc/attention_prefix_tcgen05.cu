@@ -129,12 +129,12 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     // every warp finds the work by itself: the tile's tokens, its slice of the pages, how far anybody sees
     const int per_tile = ROWS / prm.head_chunk;
     const TokenTile tile = token_tile(prm.b, blockIdx.x, per_tile);
-    const int pages = tile.count ? prm.b.pages_of(tile.group) : 0, per = pages_per_slice(pages, prm.splits);
+    const int pages = tile.pages, per = pages_per_slice(pages, prm.splits);
     const int page0 = blockIdx.z * per, page1 = min(pages, page0 + per);
     if (page0 >= page1) return;                            // (the whole CTA: nobody has allocated or asked for anything)
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
-    const int* table = prm.b.row_of(prm.b.start_of(tile.group));
+    const int* table = prm.b.row_of(tile.group_first);
     int far = -1;
     for (int i = lane; i < tile.count; i += 32)
         if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.positions[tile.first + i]);
@@ -421,6 +421,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
     __shared__ int abort_word, page_ok[MAX_STAGES];
     __shared__ float joined[OWN_ROWS][2];                  // m and l of this CTA's rows, its warps together
+    __shared__ float own_weight[OWN_ROWS][8], shared_weight[OWN_ROWS][MAX_SPLITS], inverse[OWN_ROWS];
     volatile int* abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, stages = prm.stages;
     const int slices = gridDim.z, slice = blockIdx.z;
@@ -436,14 +437,13 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     const int t = blockIdx.x, chunks = (prm.group + OWN_ROWS - 1) / OWN_ROWS;
     const int kvh = blockIdx.y / chunks, head0 = kvh * prm.group + (blockIdx.y % chunks) * OWN_ROWS;
     const int heads = min(OWN_ROWS, (kvh + 1) * prm.group - head0);
-    const int group = group_of(prm.b, t);
-    if (group < 0) {                                       // rows of no group stay as they are; the whole cluster leaves
+    const Token token = token_of(prm.b, t);
+    if (token.pages < 0) {                                 // rows of no group stay as they are; the whole cluster leaves
         pdl_wait();
         return;
     }
-    const int pages = prm.b.pages_of(group);
-    const int* table = prm.b.row_of(t);
-    const int last = table ? min(prm.b.positions[t], prm.b.max_pages * KEYS - 1) : -1;
+    const int pages = token.pages, last = token.last;
+    const int* table = token.table;
     const int own = last >= pages * KEYS ? last / KEYS + 1 - pages : 0, per = (own + slices - 1) / slices;
     const int tile0 = pages + slice * per, tile1 = min(pages + own, tile0 + per), n_tiles = max(0, tile1 - tile0);
     __syncthreads();
@@ -613,40 +613,67 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     const bool cluster = slices > 1;
     if (cluster) cluster_sync_all();
     else __syncthreads();
-    // the join: with a cluster every CTA has a share of the rows
+    // the join: with a cluster every CTA has a share of the rows.  First the parts' weights, a warp a row and a lane a part (all
+    // of them asked for at once), then the sums, eight parts' channels on the way together
     const int shared_per = pages_per_slice(pages, prm.splits), shared = shared_per ? (pages + shared_per - 1) / shared_per : 0;
     const uint32_t o_at = smem_u32(o_s), ml_at = smem_u32(joined);
+    for (int row = warp; row < heads; row += OWN_WARPS + 1) {
+        const size_t at = ((size_t)t * prm.nh + head0 + row) * prm.splits;
+        const float sink = prm.sink ? prm.sink[head0 + row] * LOG2E : -INFINITY;
+        float2 part[(MAX_SPLITS + 31) / 32], mine = make_float2(-INFINITY, 0.0f);
+        if (lane < slices) {
+            mine.x = cluster ? ld_dsmem_f32(ml_at + row * 8, lane) : joined[row][0];
+            mine.y = cluster ? ld_dsmem_f32(ml_at + row * 8 + 4, lane) : joined[row][1];
+        }
+        float top = fmaxf(sink, mine.x);
+#pragma unroll
+        for (int i = 0; i < (MAX_SPLITS + 31) / 32; ++i) {
+            part[i] = lane + 32 * i < shared ? *reinterpret_cast<const float2*>(prm.part_ml + 2 * (at + lane + 32 * i)) : make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, part[i].x);
+        }
+        top = warp_max(top);
+        const float f = part_weight(mine.x, top);
+        float sum = f * mine.y + (lane == 0 ? part_weight(sink, top) : 0.0f);
+        if (lane < slices) own_weight[row][lane] = f;
+#pragma unroll
+        for (int i = 0; i < (MAX_SPLITS + 31) / 32; ++i) {
+            const float w = part_weight(part[i].x, top);
+            if (lane + 32 * i < shared) shared_weight[row][lane + 32 * i] = w;
+            sum = fmaf(w, part[i].y, sum);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) inverse[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
+    __syncthreads();
     constexpr int LANES = HD / 4;                          // threads a row, four channels each
     for (int i = threadIdx.x; i < heads * LANES; i += OWN_THREADS) {
-        const int row = i / LANES, c = (i - row * LANES) * 4, head = head0 + row;
-        if (cluster && row % slices != slice) continue;
-        const size_t at = ((size_t)t * prm.nh + head) * prm.splits;
-        const float sink = prm.sink ? prm.sink[head] * LOG2E : -INFINITY;
-        float top = sink;
-        for (int s = 0; s < slices; ++s) top = fmaxf(top, cluster ? ld_dsmem_f32(ml_at + row * 8, s) : joined[row][0]);
-        for (int s = 0; s < shared; ++s) top = fmaxf(top, prm.part_ml[2 * (at + s)]);
-        float sum = part_weight(sink, top);
+        const int row = i / LANES, c = (i - row * LANES) * 4;
+        if ((cluster && row % slices != slice) || c >= prm.hd) continue;
+        const float* parts = prm.part_o + ((size_t)t * prm.nh + head0 + row) * prm.splits * prm.hd + c;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto add = [&](float f, const float4& x) {
             v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
         };
+        // (a part that weighs nothing may hold anything: it is not read)
+        for (int s0 = 0; s0 < shared; s0 += 8) {
+            float4 x[8];
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                f[k] = s0 + k < shared ? shared_weight[row][s0 + k] : 0.0f;
+                x[k] = f[k] != 0.0f ? *reinterpret_cast<const float4*>(parts + (size_t)(s0 + k) * prm.hd) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) add(f[k], x[k]);
+        }
         for (int s = 0; s < slices; ++s) {
-            const float f = part_weight(cluster ? ld_dsmem_f32(ml_at + row * 8, s) : joined[row][0], top);
+            const float f = own_weight[row][s];
             if (f == 0.0f) continue;
-            sum = fmaf(f, cluster ? ld_dsmem_f32(ml_at + row * 8 + 4, s) : joined[row][1], sum);
             add(f, cluster ? ld_dsmem_f32x4(o_at + (uint32_t)(row * HD + c) * 4, s) : *reinterpret_cast<const float4*>(o_s + row * HD + c));
         }
-        if (c < prm.hd)
-            for (int s = 0; s < shared; ++s) {
-                const float2 ml = *reinterpret_cast<const float2*>(prm.part_ml + 2 * (at + s));
-                const float f = part_weight(ml.x, top);
-                if (f == 0.0f) continue;
-                sum = fmaf(f, ml.y, sum);
-                add(f, *reinterpret_cast<const float4*>(prm.part_o + (at + s) * prm.hd + c));
-            }
-        if (c < prm.hd && !*abort_flag) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<uint2*>(prm.out + ((size_t)t * prm.nh + head) * prm.hd + c) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+        if (!*abort_flag) {
+            const float inv = inverse[row];
+            *reinterpret_cast<uint2*>(prm.out + ((size_t)t * prm.nh + head0 + row) * prm.hd + c) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
         }
     }
     if (cluster) cluster_sync_all();                       // nobody leaves while a peer still reads from it
