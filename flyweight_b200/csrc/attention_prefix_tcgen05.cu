@@ -1,9 +1,10 @@
 // Attention of requests that share their first pages, bfloat16, head sizes up to 128, on tensor cores.
 //
 //   prefix kernel   a CTA: 128 rows -- (token, query head of one KV head) pairs of one group -- against one slice of the group's
-//                   shared pages.  As in the prompt kernel (attention_tcgen05.cu): S = Q K^T by tcgen05.mma into one of two
-//                   buffers in tensor memory, a thread a row for the softmax, P back into its scores' columns as bfloat16
-//                   pairs, O += P V with P read from tensor memory.  m follows the running maximum only when that has grown by
+//                   shared pages, in steps of 128 keys (64 at head sizes above 64): S = Q K^T by tcgen05.mma into tensor
+//                   memory, a thread a row for the softmax, P as bfloat16 pairs into columns of its own, O += P V with P
+//                   read from tensor memory.  The scores of a step are computed while the softmax works on those of the
+//                   step before, which it holds in registers.  m follows the running maximum only when that has grown by
 //                   more than 2^8.  Leaves m (in base 2), l and O, not divided, of its slice in scratch, fp32.
 //   own kernel      a CTA: one token, up to 16 query heads of one KV head (the rows of mma.sync 16 x 8 x 16), one slice of the keys behind
 //                   the shared ones; four warps take 16 keys each of every 64-key tile that TMA brings, with a running
@@ -31,7 +32,6 @@ constexpr int ROWS = 128;        // query rows of a prefix CTA (UMMA M)
 constexpr int KEYS = PAGE;
 constexpr int SOFTMAX_WARPS = 4, PREFIX_THREADS = 64 + 32 * SOFTMAX_WARPS;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int LEAD = 2;                // the scores run this many key tiles ahead of PV
 constexpr float RESCALE_STEP = 8.0f;   // O is rescaled when a row's maximum has grown by more than 2^8
 constexpr int KV_BOX = KEYS * 128;     // 64 keys x 64 channels
 constexpr int OWN_WARPS = 4, OWN_THREADS = 32 * (OWN_WARPS + 1), OWN_ROWS = 16;
@@ -52,16 +52,18 @@ struct Params {
     int* status;
 };
 
+// Tensor memory of a CTA is 256 columns, so that two CTAs fit an SM: the scores of a step's keys, P (bfloat16 pairs), O.
 template <int HD>
 struct Layout {
-    static constexpr int BOXES = HD / 64;
+    static constexpr int STEP = HD == 64 ? 128 : 64;         // keys a step
+    static constexpr int PAGES = STEP / KEYS, BOXES = HD / 64;
     static constexpr int Q_BOX = ROWS * 128, Q_BYTES = BOXES * Q_BOX;
-    static constexpr int KV_BYTES = BOXES * KV_BOX;
-    static constexpr int STAGES = HD == 64 ? 4 : 2;          // ring slots, each one K and one V tile: two CTAs an SM
-    static constexpr int DATA = Q_BYTES + 2 * STAGES * KV_BYTES;
+    static constexpr int KV_BYTES = PAGES * BOXES * KV_BOX;  // keys (or values) of a step
+    static constexpr int SLOTS = 2;                          // of K and of V each
+    static constexpr int DATA = Q_BYTES + 2 * SLOTS * KV_BYTES;
     static constexpr int SMEM = DATA + 1024 + 256;
-    static constexpr int S_COLS = 2 * KEYS;                  // two S buffers at column 0, O behind them
-    static constexpr int TMEM_COLS = 256;
+    static constexpr int P_COL = STEP, O_COL = STEP + STEP / 2, TMEM_COLS = 256;
+    static_assert(O_COL + HD <= TMEM_COLS, "tensor memory");
 };
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -71,18 +73,48 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
+// Two floats in a register pair, for the packed fp32 instructions.
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
 }
-// A x B with A (P, bfloat16 pairs in 32-bit columns) read from tensor memory.
-__device__ __forceinline__ void umma_bf16_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                                 uint32_t accumulate) {
+__device__ __forceinline__ void unpair(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {         // NaN if one of them is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The products as the issuing thread gives them out: descriptors as their two words, of which only the lower one (the address)
+// changes, and the accumulate flag as a constant.  Everything it computes itself is paid once a tile between four warps' softmax.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void umma_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
+        : "memory");
+}
+// A (P, bfloat16 pairs in 32-bit columns) read from tensor memory.
+__device__ __forceinline__ void umma_a_tmem_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // the first row of a page's tile in the pool, seen as rows of hd entries; behind the pool's end for an id that is no page
@@ -90,36 +122,42 @@ __device__ __forceinline__ int tile_row(const Params& prm, int page, int kvh) {
     return prm.b.is_page(page) ? (page * prm.nkv + kvh) * KEYS : prm.pool_rows;
 }
 
-template <int HD>
+// CAPPED: with the soft cap's code (kept out of the other form: jumping over it costs more than a tenth of a step in fetches)
+template <int HD, bool CAPPED>
 __global__ void __launch_bounds__(PREFIX_THREADS, 2)
 prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params prm) {
     using L = Layout<HD>;
+    constexpr int STEP = L::STEP, PAGES = L::PAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = base;
     uint8_t* k_s = q_s + L::Q_BYTES;
-    uint8_t* v_s = k_s + L::STAGES * L::KV_BYTES;
-    uint64_t* full = reinterpret_cast<uint64_t*>(base + L::DATA);
-    uint64_t* empty = full + L::STAGES;
-    uint64_t* q_ready = empty + L::STAGES;
-    uint64_t* s_ready = q_ready + 1;                       // [2]: one per S buffer
-    uint64_t* p_ready = s_ready + 2;                       // [2]: P of a tile is in its S buffer
-    uint64_t* pv_ready = p_ready + 2;                      // [2]
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_ready + 2);
+    uint8_t* v_s = k_s + L::SLOTS * L::KV_BYTES;
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(base + L::DATA);      // [SLOTS] each
+    uint64_t* k_empty = k_full + L::SLOTS;
+    uint64_t* v_full = k_empty + L::SLOTS;
+    uint64_t* v_empty = v_full + L::SLOTS;
+    uint64_t* q_ready = v_empty + L::SLOTS;
+    uint64_t* s_ready = q_ready + 1;                       // the scores of a step are in tensor memory
+    uint64_t* s_taken = s_ready + 1;                       // ... and in the softmax threads' registers
+    uint64_t* p_ready = s_taken + 1;                       // P of a step is in tensor memory
+    uint64_t* pv_ready = p_ready + 1;                      // ... and in O
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_ready + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < L::STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+        for (int s = 0; s < L::SLOTS; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
         }
         mbar_init(q_ready, SOFTMAX_WARPS);
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&s_ready[b], 1);
-            mbar_init(&p_ready[b], SOFTMAX_WARPS);
-            mbar_init(&pv_ready[b], 1);
-        }
+        mbar_init(s_ready, 1);
+        mbar_init(s_taken, SOFTMAX_WARPS);
+        mbar_init(p_ready, SOFTMAX_WARPS);
+        mbar_init(pv_ready, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -138,47 +176,41 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     int far = -1;
     for (int i = lane; i < tile.count; i += 32)
         if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.positions[tile.first + i]);
-    far = __reduce_max_sync(0xffffffffu, far);
-    int n_tiles = far < 0 || !table ? 0 : min(page1, far / KEYS + 1) - page0;
-    n_tiles = n_tiles < 0 ? 0 : n_tiles;
+    far = min(__reduce_max_sync(0xffffffffu, far), page1 * KEYS - 1);
+    const int n_pages = !table || far < page0 * KEYS ? 0 : far / KEYS + 1 - page0;
+    const int n_steps = (n_pages + PAGES - 1) / PAGES;
 
     if (warp == 1) tmem_alloc(tmem_holder, L::TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
-    int asked = 0;                                         // the producer's: ring slots filled so far
+    int asked = 0;                                         // the producer's: steps asked for so far
 
     if (warp == 0) {
-        // Step t brings K tile t and V tile t - LEAD into one ring slot under one barrier: what the MMA issuer needs
-        // next at the same moment.
-        int ids = -1, ids_v = -1;                          // 32 page ids, a lane each: those of K and, a block behind, of V
-        for (int t = 0; n_tiles > 0 && t < n_tiles + LEAD; ++t) {
-            const int s = t % L::STAGES;
-            if (t % 32 == 0) {
-                ids_v = ids;
-                ids = t + lane < n_tiles ? table[page0 + t + lane] : -1;
-            }
-            const int vt = t - LEAD;
-            const int k_page = __shfl_sync(0xffffffffu, ids, t & 31);
-            const int v_page = __shfl_sync(0xffffffffu, t % 32 < LEAD ? ids_v : ids, vt & 31);
+        // a page that is none, or behind the slice's last, comes as zeros
+        int ids = -1;                                      // 32 page ids, a lane each
+        for (int t = 0; t < n_steps; ++t) {
+            const int s = t % L::SLOTS;
+            if (t * PAGES % 32 == 0) ids = t * PAGES + lane < n_pages ? table[page0 + t * PAGES + lane] : -1;
+            int row[PAGES];
+#pragma unroll
+            for (int i = 0; i < PAGES; ++i) row[i] = tile_row(prm, __shfl_sync(0xffffffffu, ids, (t * PAGES + i) & 31), kvh);
             bool ok = true;
             if (lane == 0) {
-                if (t >= L::STAGES) ok = mbar_wait(&empty[s], ((t / L::STAGES) - 1) & 1, abort_flag, 51, prm.status);
+                const uint32_t parity = ((t / L::SLOTS) - 1) & 1;
+                if (t >= L::SLOTS) ok = mbar_wait(&k_empty[s], parity, abort_flag, 51, prm.status);
                 if (ok) {
-                    const bool has_k = t < n_tiles, has_v = vt >= 0;
-                    mbar_expect_tx(&full[s], ((has_k ? 1 : 0) + (has_v ? 1 : 0)) * L::KV_BYTES);
-                    if (has_k) {
-                        const int row = tile_row(prm, k_page, kvh);
+                    mbar_expect_tx(&k_full[s], L::KV_BYTES);
 #pragma unroll
-                        for (int b = 0; b < L::BOXES; ++b)
-                            tma_load_2d(k_s + (size_t)s * L::KV_BYTES + b * KV_BOX, &map_k, &full[s], b * 64, row);
-                    }
-                    if (has_v) {
-                        const int row = tile_row(prm, v_page, kvh);
+                    for (int i = 0; i < PAGES * L::BOXES; ++i)
+                        tma_load_2d(k_s + (size_t)s * L::KV_BYTES + i * KV_BOX, &map_k, &k_full[s], i / PAGES * 64, row[i % PAGES]);
+                    if (t >= L::SLOTS) ok = mbar_wait(&v_empty[s], parity, abort_flag, 54, prm.status);
+                    if (ok) {
+                        mbar_expect_tx(&v_full[s], L::KV_BYTES);
 #pragma unroll
-                        for (int b = 0; b < L::BOXES; ++b)
-                            tma_load_2d(v_s + (size_t)s * L::KV_BYTES + b * KV_BOX, &map_v, &full[s], b * 64, row);
+                        for (int i = 0; i < PAGES * L::BOXES; ++i)
+                            tma_load_2d(v_s + (size_t)s * L::KV_BYTES + i * KV_BOX, &map_v, &v_full[s], i / PAGES * 64, row[i % PAGES]);
                     }
                     ++asked;
                 }
@@ -186,61 +218,58 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
         }
     } else if (warp == 1) {
-        if (lane == 0 && n_tiles > 0) {
-            constexpr uint32_t idesc_qk = make_idesc_mn(ROWS, KEYS);
+        if (lane == 0 && n_steps > 0) {
+            constexpr uint32_t idesc_qk = make_idesc_mn(ROWS, STEP);
             constexpr uint32_t idesc_pv = make_idesc_mn(ROWS, HD) | IDESC_B_MN_MAJOR;
-            const uint32_t tmem_pv = tmem_base + L::S_COLS, q_addr = smem_u32(q_s);
             const int k_steps = (prm.hd + UMMA_K - 1) / UMMA_K;
-            // S of tile j goes to buffer j & 1.  One thread issues everything, so a commit also covers every product
-            // issued before it: when S of tile j is ready, PV of tile j - 2 has read its P, which lay in that buffer.
+            const uint64_t q_desc = make_smem_desc(smem_u32(q_s)), k_desc = make_smem_desc(smem_u32(k_s));
+            const uint64_t v_desc = make_smem_desc_mn_major(smem_u32(v_s), KV_BOX);
+            const uint32_t q_lo = (uint32_t)q_desc, k_lo0 = (uint32_t)k_desc, v_lo0 = (uint32_t)v_desc;
+            const uint32_t k_hi = (uint32_t)(k_desc >> 32), v_hi = (uint32_t)(v_desc >> 32);
             bool ok = mbar_wait(q_ready, 0, abort_flag, 52, prm.status);
-            auto wait_step = [&](int u) {
-                const int s = u % L::STAGES;
-                ok = ok && mbar_wait(&full[s], (u / L::STAGES) & 1, abort_flag, 53, prm.status);
+            auto issue_qk = [&](int j) {
+                const int s = j % L::SLOTS;
+                ok = ok && mbar_wait(&k_full[s], (j / L::SLOTS) & 1, abort_flag, 53, prm.status);
+                if (ok && j > 0) ok = mbar_wait(s_taken, (j - 1) & 1, abort_flag, 59, prm.status);
+                if (!ok) return;
                 tc_fence_after();
-                return s;
-            };
-            auto issue_qk = [&](int j, int s) {
-                const uint32_t k_addr = smem_u32(k_s + (size_t)s * L::KV_BYTES);
-                for (int kk = 0; kk < k_steps; ++kk) {
-                    const uint64_t a = make_smem_desc(q_addr + (kk >> 2) * L::Q_BOX) + 2 * (kk & 3);
-                    const uint64_t b = make_smem_desc(k_addr + (kk >> 2) * KV_BOX) + 2 * (kk & 3);
-                    umma_bf16(tmem_base + (j & 1) * KEYS, a, b, idesc_qk, kk > 0 ? 1u : 0u);
-                }
-                umma_commit(&s_ready[j & 1]);
-            };
-            int u = 0;
-            for (int t = 0; t < LEAD && ok; ++t, ++u) {               // the steps that bring no V yet
-                const int s = wait_step(u);
-                if (!ok) break;
-                if (t < n_tiles) issue_qk(t, s);
-                umma_commit(&empty[s]);
-            }
-            for (int j = 0; j < n_tiles && ok; ++j, ++u) {
-                ok = mbar_wait(&p_ready[j & 1], (j >> 1) & 1, abort_flag, 55, prm.status);
-                const int s = wait_step(u);
-                if (!ok) break;
-                const uint32_t v_addr = smem_u32(v_s + (size_t)s * L::KV_BYTES);
+                const uint32_t k_lo = k_lo0 + s * (L::KV_BYTES >> 4);
 #pragma unroll
-                for (int kk = 0; kk < KEYS / UMMA_K; ++kk) {
-                    const uint64_t b = make_smem_desc_mn_major(v_addr + kk * 2048, KV_BOX);    // 16 keys: two 8-row groups
-                    umma_bf16_a_tmem(tmem_pv, tmem_base + (j & 1) * KEYS + kk * 8, b, idesc_pv, j > 0 || kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < HD / UMMA_K; ++kk) {           // 16 channels: 32 bytes along the row, four to a box
+                    const uint32_t qa = q_lo + (kk >> 2) * (L::Q_BOX >> 4) + 2 * (kk & 3), ka = k_lo + (kk >> 2) * (PAGES * KV_BOX >> 4) + 2 * (kk & 3);
+                    if (kk == 0) umma_lo<false>(tmem_base, qa, ka, k_hi, idesc_qk);
+                    else if (kk < k_steps) umma_lo<true>(tmem_base, qa, ka, k_hi, idesc_qk);
                 }
-                umma_commit(&pv_ready[j & 1]);
-                if (j + LEAD < n_tiles) issue_qk(j + LEAD, s);
-                umma_commit(&empty[s]);
+                umma_commit(s_ready);
+                umma_commit(&k_empty[s]);
+            };
+            issue_qk(0);
+            for (int j = 0; j < n_steps && ok; ++j) {
+                // the next scores while the softmax works on this step's, as soon as these are in its registers
+                if (j + 1 < n_steps) issue_qk(j + 1);
+                const int s = j % L::SLOTS;
+                ok = ok && mbar_wait(&v_full[s], (j / L::SLOTS) & 1, abort_flag, 63, prm.status);
+                ok = ok && mbar_wait(p_ready, j & 1, abort_flag, 55, prm.status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t v_lo = v_lo0 + s * (L::KV_BYTES >> 4);
+#pragma unroll
+                for (int kk = 0; kk < STEP / UMMA_K; ++kk)            // 16 keys: 2048 bytes of V, 8 columns of P
+                    umma_a_tmem_lo(tmem_base + L::O_COL, tmem_base + L::P_COL + kk * 8,
+                                   v_lo + ((kk >> 2) * KV_BOX >> 4) + (kk & 3) * (2048 >> 4), v_hi, idesc_pv, kk > 0 ? 1u : (uint32_t)j);
+                umma_commit(pv_ready);
+                umma_commit(&v_empty[s]);
             }
         }
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane, swz = row & 7;
-        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + L::S_COLS;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
         const int t_in = row / prm.head_chunk, h_in = row - t_in * prm.head_chunk;
         const bool valid = t_in < tile.count && h_in < heads;
         const int tok = tile.first + (valid ? t_in : 0), head = kvh * prm.group + head0 + (valid ? h_in : 0);
-        const int hi = valid && prm.b.row_of(tok) ? prm.b.positions[tok] : -1;
-        bool ok = true;
+        const int hi = min(far, valid && prm.b.row_of(tok) ? prm.b.positions[tok] : -1);
         float m = -INFINITY, l = 0.0f;
-        if (n_tiles > 0) {
+        if (n_steps > 0) {
             const __nv_bfloat16* q_row = prm.q + ((size_t)tok * prm.nh + head) * prm.hd;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
@@ -251,115 +280,138 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         }
-        int ids = -1;
-        for (int j = 0; j < n_tiles; ++j) {
-            const int key0 = (page0 + j) * KEYS, buf = j & 1;
-            if (j % 32 == 0) ids = j + lane < n_tiles ? table[page0 + j + lane] : -1;
-            const bool is_page = prm.b.is_page(__shfl_sync(0xffffffffu, ids, j & 31));
-            ok = mbar_wait(&s_ready[buf], (j >> 1) & 1, abort_flag, 56, prm.status);
-            ok = __all_sync(0xffffffffu, ok);              // tcgen05.ld needs the whole warp
-            if (!ok) break;
+        // from which key on some row of this warp does not see everything, and whether all of the slice's pages are pages
+        const int whole_to = (int)__reduce_min_sync(0xffffffffu, (unsigned)(valid ? hi + 1 : 0x7fffffff));
+        bool all_pages = true;
+        for (int i = lane; i < n_pages; i += 32) all_pages &= prm.b.is_page(table[page0 + i]);
+        all_pages = __all_sync(0xffffffffu, all_pages);
+        const unsigned long long scale2 = pair(prm.scale_log2, prm.scale_log2);
+        unsigned long long sum2 = 0;
+        for (int j = 0; j < n_steps; ++j) {
+            const int key0 = (page0 + j * PAGES) * KEYS;
+            // (nothing goes by the answers of this loop's waits: after one that gave up every other ends at its first poll, and nobody
+            // stores)
+            mbar_wait(s_ready, j & 1, abort_flag, 56, prm.status);
+            __syncwarp();                                  // tcgen05.ld needs the whole warp
             tc_fence_after();
-            float sc[KEYS];
-            tmem_ld64(lane_addr + buf * KEYS, sc);
+            float sc[STEP];
+            if constexpr (STEP == 128) tmem_ld128(lane_addr, sc);
+            else tmem_ld64(lane_addr, sc);
             tc_fence_before();
-            if (prm.cap_pre != 0.0f) {
-                // a warp whose scores of this tile all lie far below the cap takes the polynomial: it spares the
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_taken);
+            if constexpr (CAPPED) {
+                // a warp whose scores of this step all lie far below the cap takes the polynomial: it spares the
                 // special-function unit, which the exponentials need
                 float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < KEYS; ++i) {
+                for (int i = 0; i < STEP; ++i) {
                     sc[i] *= prm.cap_pre;
                     top = fmaxf(top, fabsf(sc[i]));
                 }
                 if (__all_sync(0xffffffffu, top <= TANH_SMALL)) {
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) sc[i] = prm.cap_unit * tanh_small_f32(sc[i]);
+                    for (int i = 0; i < STEP; ++i) sc[i] = prm.cap_unit * tanh_small_f32(sc[i]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) sc[i] = prm.cap_unit * tanh_fast_f32(sc[i]);
+                    for (int i = 0; i < STEP; ++i) sc[i] = prm.cap_unit * tanh_fast_f32(sc[i]);
                 }
             }
-            // a tile every row sees whole needs no mask (rows without a token are never stored)
-            if (!is_page || !__all_sync(0xffffffffu, !valid || key0 + KEYS - 1 <= hi)) {
-                const int last = is_page ? hi : -1;
+            // a step every row sees whole needs no mask (rows without a token are never stored)
+            const bool whole = all_pages && key0 + STEP <= whole_to;
+            if (__builtin_expect(!whole, 0)) {
 #pragma unroll
-                for (int i = 0; i < KEYS; ++i) sc[i] = key0 + i <= last ? sc[i] : -INFINITY;
+                for (int i = 0; i < PAGES; ++i) {
+                    const int p = j * PAGES + i;
+                    const int last = p < n_pages && prm.b.is_page(table[page0 + p]) ? hi : -1;
+#pragma unroll
+                    for (int k = 0; k < KEYS; ++k) sc[i * KEYS + k] = key0 + i * KEYS + k <= last ? sc[i * KEYS + k] : -INFINITY;
+                }
             }
-            // four interleaved chains each for the maximum and the sum: a fixed order, a quarter of the latency
+            // four interleaved chains for the maximum, two values a link
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < KEYS; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[i]);
-            const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * prm.scale_log2;
-            const bool moved = tile_max > m + RESCALE_STEP;          // also: the row's first keys (m = -inf)
+            for (int i = 0; i < STEP; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], sc[i], sc[i + 1]);
+            const float step_max = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * prm.scale_log2;
+            const bool moved = step_max > m + RESCALE_STEP;          // also: the row's first keys (m = -inf)
             float factor = 1.0f;
             if (moved) {
-                factor = ex2(m - tile_max);                          // 2^(-inf) = 0 for the first keys
-                m = tile_max;
+                factor = ex2(m - step_max);                          // 2^(-inf) = 0 for the first keys
+                m = step_max;
                 l *= factor;
+                sum2 = fma2(sum2, pair(factor, factor), 0);
             }
-            if (j > 0 && __any_sync(0xffffffffu, moved)) {
-                // every PV so far has landed in O; scale this warp's rows (by exactly 1 where nothing moved)
-                ok = mbar_wait(&pv_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, 58, prm.status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+            if (j > 0) {
+                // PV of the step before has read its P, whose columns this one's takes, and landed in O
+                mbar_wait(pv_ready, (j - 1) & 1, abort_flag, 58, prm.status);
+                __syncwarp();
                 tc_fence_after();
+                if (__builtin_expect(__any_sync(0xffffffffu, moved), 0)) {
+                    // scale this warp's rows (by exactly 1 where nothing moved)
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        float v[16];
+                        tmem_ld16(lane_addr + L::O_COL + c0, v);
 #pragma unroll
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    float v[32];
-                    tmem_ld32(o_addr + c0, v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= factor;
-                    tmem_st32(o_addr + c0, v);
+                        for (int i = 0; i < 16; ++i) v[i] *= factor;
+                        tmem_st16_async(lane_addr + L::O_COL + c0, v);
+                    }
+                    tmem_st_wait();
                 }
-                tc_fence_before();
             }
             const float zero = m == -INFINITY ? 0.0f : m;            // a row that has seen no key yet
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            float packed[KEYS / 2];
+            const unsigned long long minus = pair(-zero, -zero);
 #pragma unroll
-            for (int i = 0; i < KEYS; i += 2) {
-                const float p0 = ex2(fmaf(sc[i], prm.scale_log2, -zero));         // masked: 2^(-inf) = 0
-                const float p1 = ex2(fmaf(sc[i + 1], prm.scale_log2, -zero));
-                sum[i & 3] += p0;
-                sum[(i + 1) & 3] += p1;
-                packed[i >> 1] = __uint_as_float(pack2(p0, p1));
+            for (int c0 = 0; c0 < STEP; c0 += 32) {
+                float packed[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float p0, p1;
+                    unpair(fma2(pair(sc[c0 + i], sc[c0 + i + 1]), scale2, minus), p0, p1);
+                    p0 = ex2(p0), p1 = ex2(p1);                      // masked: 2^(-inf) = 0
+                    sum2 = add2(sum2, pair(p0, p1));
+                    packed[i >> 1] = __uint_as_float(pack2(p0, p1));
+                }
+                tmem_st16_async(lane_addr + L::P_COL + c0 / 2, packed);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            // P goes back into the columns its scores came from: the buffer's last reader, PV of the tile before the last,
-            // had completed when this tile's S was ready
-            tmem_st32(lane_addr + buf * KEYS, packed);
+            if (!(step_max < INFINITY)) l = __int_as_float(0x7fffffff);     // an infinity or NaN among the scores
+            tmem_st_wait();
             tc_fence_before();
-            const int seen = far + 1 - key0;                          // keys of this tile anybody may see
-            if (seen < KEYS) {
-                // only the last tile: clear the V rows behind it (whole 128-byte rows of every box)
-                const int u = j + LEAD, s = u % L::STAGES;            // the step that brought this V tile
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (u / L::STAGES) & 1, abort_flag, 57, prm.status));
+            const int seen = far + 1 - key0;                          // keys of this step anybody may see
+            if (__builtin_expect(seen < STEP, 0)) {
+                // only the last step: clear the V rows behind them (whole 128-byte rows of every box)
+                const int s = j % L::SLOTS;
+                mbar_wait(&v_full[s], (j / L::SLOTS) & 1, abort_flag, 57, prm.status);
                 uint8_t* v_tile = v_s + (size_t)s * L::KV_BYTES;
-                const int chunks = (KEYS - seen) * 8;
+                const int chunks = (STEP - seen) * 8;
                 for (int b = 0; b < L::BOXES; ++b)
                     for (int i = threadIdx.x - 64; i < chunks; i += 32 * SOFTMAX_WARPS)
-                        *reinterpret_cast<uint4*>(v_tile + b * KV_BOX + seen * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(v_tile + b * PAGES * KV_BOX + seen * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async();                                  // the cleared rows, for the tensor core
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[buf]);
+            if (lane == 0) mbar_arrive(p_ready);
         }
-        if (ok && n_tiles > 0) {
-            const int last = n_tiles - 1;
-            ok = mbar_wait(&pv_ready[last & 1], (last >> 1) & 1, abort_flag, 60, prm.status);
-            ok = __all_sync(0xffffffffu, ok);
+        {
+            float a, b;
+            unpair(sum2, a, b);
+            l += a + b;
+        }
+        bool ok = true;
+        if (n_steps > 0) {
+            ok = mbar_wait(pv_ready, (n_steps - 1) & 1, abort_flag, 60, prm.status);
+            ok = __all_sync(0xffffffffu, ok && !*abort_flag);
         }
         if (ok) {
             tc_fence_after();
             const size_t at = ((size_t)tok * prm.nh + head) * prm.splits + blockIdx.z;
             // (a slice that a row sees nothing of is left out by its m: its O is not read)
             if (valid) *reinterpret_cast<float2*>(prm.part_ml + 2 * at) = make_float2(m, l);
-            if (n_tiles > 0) {
+            if (n_steps > 0) {
 #pragma unroll
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     float v[32];
-                    tmem_ld32(o_addr + c0, v);
+                    tmem_ld32(lane_addr + L::O_COL + c0, v);
                     if (valid) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4)
@@ -375,9 +427,10 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag)
-        for (int s = 0; s < L::STAGES && s < asked; ++s) {           // copies still in flight land first
-            const uint32_t last = (uint32_t)((asked - 1 - s) / L::STAGES) & 1;
-            for (unsigned spin = 0; spin < WAIT_LIMIT && !mbar_test(&full[s], last); ++spin) __nanosleep(64);
+        for (int s = 0; s < L::SLOTS && s < asked; ++s) {            // copies still in flight land first
+            const uint32_t last = (uint32_t)((asked - 1 - s) / L::SLOTS) & 1;
+            for (unsigned spin = 0; spin < WAIT_LIMIT && !mbar_test(&k_full[s], last); ++spin) __nanosleep(64);
+            for (unsigned spin = 0; spin < WAIT_LIMIT && !mbar_test(&v_full[s], last); ++spin) __nanosleep(64);
         }
     if (warp == 1) tmem_dealloc(tmem_base, L::TMEM_COLS);
 }
@@ -682,17 +735,19 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
 template <int HD>
 int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int own_slices, cudaStream_t stream) {
     using L = Layout<HD>;
-    auto prefix = prefix_tcgen05_kernel<HD>;
+    auto plain = prefix_tcgen05_kernel<HD, false>;
+    auto capped = prefix_tcgen05_kernel<HD, true>;
     auto own = own_kernel<HD>;
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(prefix, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(plain, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(capped, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
     const long tiles = most_token_tiles(prm.b.T, prm.b.n_groups, ROWS / prm.head_chunk);
-    fwb::pdl(prefix, dim3((unsigned)tiles, prm.nkv * prm.head_chunks, prm.splits), PREFIX_THREADS, L::SMEM, stream)(map_k, map_v, prm);
+    fwb::pdl(prm.cap_pre != 0.0f ? capped : plain, dim3((unsigned)tiles, prm.nkv * prm.head_chunks, prm.splits), PREFIX_THREADS, L::SMEM, stream)(map_k, map_v, prm);
     int e = fwb_launch_status();
     if (e) return e;
     prm.stages = HD == 64 ? 3 : 2;
