@@ -95,6 +95,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {         // Na
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
 // The products as the issuing thread gives them out: descriptors as their two words, of which only the lower one (the address)
 // changes, and the accumulate flag as a constant.  Everything it computes itself is paid once a tile between four warps' softmax.
 template <bool ACCUMULATE>
