@@ -86,19 +86,21 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
     const int* table = prm.b.row_of(tile.group_first);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, rows = tile.count * prm.head_chunk;
+    const bool works = (threadIdx.x >> 5) * 8 < rows;  // a warp has eight rows; those without any only fetch
 
-    for (int i = threadIdx.x; i < ROWS * pitch; i += THREADS) {
+    for (int i = threadIdx.x; i < rows * pitch; i += THREADS) {
         const int r = i / pitch, c = i - r * pitch, tok = r / prm.head_chunk, h = r % prm.head_chunk;
-        const bool live = tok < tile.count && h < heads && c < hd;
+        const bool live = h < heads && c < hd;
         q_s[i] = live ? to_f32(reinterpret_cast<const T*>(prm.q)[((size_t)(tile.first + tok) * prm.nh + kvh * prm.group + head0 + h) * hd + c]) : 0.0f;
     }
-    int last[4];                                       // the last key each of this thread's rows sees
+    int last[4], whole_to = 0x7fffffff;                // the last key each of this thread's rows sees; the least of them
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty * 4 + i, tok = r / prm.head_chunk;
-        const bool live = tok < tile.count && r % prm.head_chunk < heads && prm.b.row_of(tile.first + tok);
-        last[i] = live ? prm.b.positions[tile.first + tok] : -1;
+        const bool is_row = tok < tile.count && r % prm.head_chunk < heads;
+        last[i] = is_row && prm.b.row_of(tile.first + tok) ? prm.b.positions[tile.first + tok] : -1;
+        if (is_row) whole_to = min(whole_to, last[i]);
     }
     float m[4], l[4], acc[4][COLS][4];
 #pragma unroll
@@ -115,7 +117,9 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
         __syncthreads();
         load_tiles<T>(prm, k_s, pitch, v_s, COLS * 64, (size_t)page * prm.nkv + kvh, PAGE);
         __syncthreads();
+        if (!works) continue;
         float s[4][4] = {};
+#pragma unroll 2
         for (int d = 0; d < hd; d += 4) {               // (channels behind the last are zero in both)
             float4 a[4], b[4];
 #pragma unroll
@@ -157,6 +161,9 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
                 for (int j = 0; j < 4; ++j) acc[i][c][j] *= factor;
         }
         __syncwarp();                                  // a row's sixteen threads are one half of a warp
+        // a key that a row does not see weighs nothing, whatever its value holds; where all four rows see all keys nobody asks
+        const bool whole = __all_sync(0xffffffffu, p * PAGE + PAGE - 1 <= whole_to);
+#pragma unroll 4
         for (int key = 0; key < PAGE; ++key) {
             float w[4];
 #pragma unroll
@@ -166,11 +173,9 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
                 const float4 x = *reinterpret_cast<const float4*>(v_s + key * COLS * 64 + c * 64 + tx * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // a key no row may see weighs nothing, whatever its value holds
-                    acc[i][c][0] = w[i] != 0.0f ? fmaf(w[i], x.x, acc[i][c][0]) : acc[i][c][0];
-                    acc[i][c][1] = w[i] != 0.0f ? fmaf(w[i], x.y, acc[i][c][1]) : acc[i][c][1];
-                    acc[i][c][2] = w[i] != 0.0f ? fmaf(w[i], x.z, acc[i][c][2]) : acc[i][c][2];
-                    acc[i][c][3] = w[i] != 0.0f ? fmaf(w[i], x.w, acc[i][c][3]) : acc[i][c][3];
+                    if (!whole && w[i] == 0.0f) continue;
+                    acc[i][c][0] = fmaf(w[i], x.x, acc[i][c][0]), acc[i][c][1] = fmaf(w[i], x.y, acc[i][c][1]);
+                    acc[i][c][2] = fmaf(w[i], x.z, acc[i][c][2]), acc[i][c][3] = fmaf(w[i], x.w, acc[i][c][3]);
                 }
             }
         }

@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import lib, ops
+from .lib import KernelError, check_tensor
 
 SM_COUNT = 148
 CLUSTER_MERGE_CTAS = 1024
@@ -295,25 +296,34 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
 
     All arrays are read on the device, so a captured step replays with other groups.  ``shared_pages`` and ``own_pages`` only
     say what the work is cut for (the longest shared part, the longest own part; default: the block table's width)."""
-    from .lib import KernelError, c_float, check_tensor, is_bf16, ptr, stream
-    check_tensor("q", q)
-    check_tensor("k pool", k_pool, q.dtype)
-    check_tensor("v pool", v_pool, q.dtype, k_pool.shape)
-    if q.dim() != 2 or k_pool.dim() != 4 or k_pool.shape[2] != 64:
-        raise KernelError("q must be [tokens][heads * head_dim], the pools [pages][kv_heads][64][head_dim]")
+    dtype = q.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float32) or q.dim() != 2 or not q.is_cuda or not q.is_contiguous():
+        check_tensor("q", q)
+        raise KernelError(f"q must be a float32 or bfloat16 matrix, got {dtype} {tuple(q.shape)}")
+    T, columns = q.shape
+    if k_pool.dim() != 4 or k_pool.shape[2] != 64:
+        raise KernelError(f"the pools must be [pages][kv_heads][64][head_dim], got {tuple(k_pool.shape)}")
+    check_tensor("k pool", k_pool, dtype)
+    check_tensor("v pool", v_pool, dtype, k_pool.shape)
     num_pages, n_kv, _, head_dim = k_pool.shape
-    T = q.shape[0]
-    if n_heads <= 0 or n_heads % n_kv or q.shape[1] != n_heads * head_dim:
-        raise KernelError(f"q has {q.shape[1]} columns, expected {n_heads} heads of {head_dim} over {n_kv} KV heads")
+    if n_heads <= 0 or n_heads % n_kv or columns != n_heads * head_dim:
+        raise KernelError(f"q has {columns} columns, expected {n_heads} heads of {head_dim} over {n_kv} KV heads")
     if head_dim > 256:
         raise KernelError(f"head sizes up to 256, got {head_dim}")
     for name, tensor in (("positions", positions), ("tok_seg", tok_seg), ("block table", block_table),
                          ("group starts", group_start), ("group pages", group_pages)):
-        check_tensor(name, tensor, torch.int32)
+        if tensor.dtype is not torch.int32 or not tensor.is_cuda or not tensor.is_contiguous():
+            check_tensor(name, tensor, torch.int32)
+    device = lib._device_index()
+    for name, tensor in (("q", q), ("k pool", k_pool), ("v pool", v_pool), ("positions", positions), ("tok_seg", tok_seg),
+                         ("block table", block_table), ("group starts", group_start), ("group pages", group_pages)):
+        if tensor.get_device() != device:
+            raise KernelError(f"{name} is on {tensor.device}, the kernels are launched on cuda:{device}")
     if positions.numel() < T or tok_seg.numel() < T:
         raise KernelError(f"{T} tokens need a position and a request each")
     if block_table.dim() != 2 or block_table.numel() == 0:
         raise KernelError("the block table must be [requests][pages]")
+    requests, width = block_table.shape
     groups = group_pages.numel()
     if group_start.numel() != groups + 1:
         raise KernelError(f"{groups} groups need {groups + 1} starts, got {group_start.numel()}")
@@ -324,16 +334,19 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     if out is None:
         out = torch.empty_like(q)
     else:
-        check_tensor("attention output", out, q.dtype, q.shape)
+        check_tensor("attention output", out, dtype, q.shape)
     if T == 0 or groups == 0:
         return out
-    width = block_table.shape[1]
-    wide = q.dtype == torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
+    wide = dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
     splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, width if shared_pages is None else min(width, shared_pages),
                                        width if own_pages is None else own_pages, wide)
-    part_o = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
-    part_ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
-    lib.call("fwb_attention_prefix", ptr(q), ptr(k_pool), ptr(v_pool), is_bf16(q), ptr(positions), ptr(tok_seg), ptr(block_table),
-             block_table.shape[0], width, num_pages, ptr(group_start), ptr(group_pages), groups, ptr(part_o), ptr(part_ml),
-             ptr(out), T, n_heads, n_kv, head_dim, splits, own, c_float(scale), ptr(sink), c_float(softcap), stream(), launches=2)
+    # every slice's maximum and sum, then (on a border of 16 bytes) its O
+    rows = T * n_heads * splits
+    rows += rows & 1
+    scratch = torch.empty(rows * (head_dim + 2), dtype=torch.float32, device=q.device)
+    part_ml = scratch.data_ptr()
+    lib.call("fwb_attention_prefix", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), 1 if dtype is torch.bfloat16 else 0,
+             positions.data_ptr(), tok_seg.data_ptr(), block_table.data_ptr(), requests, width, num_pages, group_start.data_ptr(),
+             group_pages.data_ptr(), groups, part_ml + 8 * rows, part_ml, out.data_ptr(), T, n_heads, n_kv, head_dim,
+             splits, own, scale, lib.ptr(sink), softcap, lib.stream(), launches=2)
     return out

@@ -137,12 +137,14 @@ def _run(x, w: Int8Matrix, out, out_dtype, addend, features: int, epilogue: int,
     if K != w.columns:
         raise KernelError(f"8-bit product: input has {K} columns, weight has {w.columns}")
     _here("weight", w._buffer)
-    if out is None:
-        out = torch.empty((M, features), dtype=out_dtype, device=w._buffer.device)
-    else:
-        check_tensor("product output", out, out_dtype, (M, features))
     if addend is not None:
         check_tensor("product addend", addend, _FP32, (M, features))
+        if out is None:
+            out = torch.empty_like(addend)
+    if out is None:
+        out = torch.empty((M, features), dtype=out_dtype, device=w._buffer.device)
+    elif out is not addend:
+        check_tensor("product output", out, out_dtype, (M, features))
     if ready:
         _here("rows", x._buffer)
         _product(x, w, out, addend, features, epilogue, limit)
