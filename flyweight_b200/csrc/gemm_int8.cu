@@ -594,7 +594,7 @@ int launch(Params prm, int tile, int splits, cudaStream_t stream) {
 // 4.2 (6.0), gated 32 x 1024 x 4608 5.1 (7.1), but 32 x 8192 x 2048 11.4 (9.4), gated 32 x 2048 x 8192 15.1 (12.5).  Beyond 512 tokens
 // the pairs win.  Between, a launch takes about 3 us (pairs 3 to 6) and, for every 128 k that a CTA walks, 0.36 (0.63 with a gate;
 // pairs 0.29 and 0.65, a further round of tiles with a gate 0.35 to 0.45) -- a latency, or with every SM at it HBM's rate -- then its stores, and 1.6 us for the
-// cluster that adds slices (3.1 with eight): 64 x 8192 x 2048 in 32-token tiles 27.1 16.6 10.9 11.1 with 1 2 4 8 slices, in 64-token
+// cluster that adds slices (3 to 6 with eight): 64 x 8192 x 2048 in 32-token tiles 27.1 16.6 10.9 11.1 with 1 2 4 8 slices, in 64-token
 // tiles 27.1 17.0 11.5 12.2, pairs 22.8; 256 x 8192 x 2048 in 128-token tiles 28.8 19.0 14.3, pairs 23.6; gated 256 x 1024 x 4608 in
 // 128-token tiles 10.2, pairs 9.8.  CTAs beyond what the SMs hold at once wait for a round of their own: gated 64 x 2048 x 8192 in
 // 128 CTAs 14.5, in 256 22.7; clusters are not taken for that.
@@ -620,12 +620,14 @@ void choose(int M, int N, int K, bool gated, int* tile, int* splits) {
         const int used = M < t ? M : t;
         for (int s = 1; s <= 8 && (s == 1 || n_kb >= 2 * s); s *= 2) {
             const long ctas = (long)((N + BM - 1) / BM) * ((M + t - 1) / t) * s;
-            // CTAs the SMs hold at once, by shared memory; clusters of four and eight leave SMs of a GPC over
+            // CTAs the SMs hold at once, by shared memory; clusters leave SMs of a GPC over, and beyond that would wait for one another
             const int kb = (n_kb + s - 1) / s, ring = (kb < 4 ? kb : 4) * (halves * A_BYTES + t * BK8), sums = s > 1 ? halves * t * BM * 4 : 0;
-            const long held = 227 * 1024 / ((ring > sums ? ring : sums) + 2048) * (s < 4 ? SM_COUNT : SM_COUNT * 7 / 8);
-            if (s > 1 && ctas > (s == 8 ? SM_COUNT : held)) continue;          // clusters wait for one another's places
-            const float walk = kb * (gated ? 0.63f : 0.36f) * (ctas > SM_COUNT && ctas <= held ? 1.17f : 1.0f);
-            consider(t, s, 3.0f + ((ctas + held - 1) / held) * (walk + 0.016f * used) + (s == 1 ? 0.0f : s < 8 ? 1.6f : 3.1f));
+            const long held = (s > 1 && t == 128 ? 1 : 227 * 1024 / ((ring > sums ? ring : sums) + 2048)) * (s > 1 ? SM_COUNT * 7 / 8 : SM_COUNT);
+            if (s > 1 && ctas > (held < 2 * SM_COUNT * 7 / 8 ? held : 2 * SM_COUNT * 7 / 8)) continue;
+            const bool crowded = ctas > SM_COUNT && ctas <= held;
+            const float walk = kb * (gated ? 0.63f : 0.36f) * (crowded ? 1.17f : 1.0f);
+            const float join = s == 1 ? 0.0f : (s < 8 ? 1.6f : t == 32 ? 3.1f : 6.0f) + (crowded ? 2.0f : 0.0f);
+            consider(t, s, 3.0f + ((ctas + held - 1) / held) * (walk + 0.016f * used) + join);
         }
     }
     for (int t = 128; t <= 256; t *= 2) {
