@@ -9,7 +9,7 @@
 //   own kernel      a CTA: one token, up to 16 query heads of one KV head (the rows of mma.sync 16 x 8 x 16), one slice of the keys behind
 //                   the shared ones; four warps take 16 keys each of every 64-key tile that TMA brings, with a running
 //                   maximum and sum each.  The warps' results meet in shared memory, the slices' in a cluster, the shared
-//                   part's slices from scratch: m = max m_i, O = sum 2^(m_i - m) O_i, l likewise; a sink joins m and l.
+//                   part's slices from scratch (or, alone, all keys are its own): m = max m_i, O = sum 2^(m_i - m) O_i, l likewise; a sink joins m and l.
 //
 // The shared keys are thus read once for 128 rows.  The own kernel starts as the prefix kernel's CTAs leave and waits for them
 // only ahead of the join: the prefix kernel lets it start when it has itself waited for the kernel in front, so everything that the own
@@ -49,6 +49,7 @@ struct Params {
                                  // cap_unit = cap / scale, so that the scale that follows gives cap * tanh(score / cap); 0: off
     int pool_rows;               // num_pages * nkv * 64: a row from here on is fetched as zeros
     int stages;                  // own kernel: depth of the ring
+    int alone;                   // own kernel: no prefix kernel in front, it walks the shared pages too
     int* status;
 };
 
@@ -490,6 +491,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (prm.alone) pdl_wait();
     pdl_launch_dependents();     // (the kernel behind waits for all of this one)
     const int t = blockIdx.x, chunks = (prm.group + OWN_ROWS - 1) / OWN_ROWS;
     const int kvh = blockIdx.y / chunks, head0 = kvh * prm.group + (blockIdx.y % chunks) * OWN_ROWS;
@@ -499,7 +501,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         pdl_wait();
         return;
     }
-    const int pages = token.pages, last = token.last;
+    const int pages = prm.alone ? 0 : token.pages, last = token.last;
     const int* table = token.table;
     const int own = last >= pages * KEYS ? last / KEYS + 1 - pages : 0, per = (own + slices - 1) / slices;
     const int tile0 = pages + slice * per, tile1 = min(pages + own, tile0 + per), n_tiles = max(0, tile1 - tile0);
@@ -672,7 +674,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     else __syncthreads();
     // the join: with a cluster every CTA has a share of the rows.  First the parts' weights, a warp a row and a lane a part (all
     // of them asked for at once), then the sums, eight parts' channels on the way together
-    const int shared_per = pages_per_slice(pages, prm.splits), shared = shared_per ? (pages + shared_per - 1) / shared_per : 0;
+    const int shared_per = pages ? pages_per_slice(pages, prm.splits) : 0, shared = pages ? (pages + shared_per - 1) / shared_per : 0;
     const uint32_t o_at = smem_u32(o_s), ml_at = smem_u32(joined);
     for (int row = warp; row < heads; row += OWN_WARPS + 1) {
         const size_t at = ((size_t)t * prm.nh + head0 + row) * prm.splits;
@@ -750,8 +752,9 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int o
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
+    prm.alone = prm.splits == 0;
     const long tiles = most_token_tiles(prm.b.T, prm.b.n_groups, ROWS / prm.head_chunk);
-    fwb::pdl(prm.cap_pre != 0.0f ? capped : plain, dim3((unsigned)tiles, prm.nkv * prm.head_chunks, prm.splits), PREFIX_THREADS, L::SMEM, stream)(map_k, map_v, prm);
+    if (!prm.alone) fwb::pdl(prm.cap_pre != 0.0f ? capped : plain, dim3((unsigned)tiles, prm.nkv * prm.head_chunks, prm.splits), PREFIX_THREADS, L::SMEM, stream)(map_k, map_v, prm);
     int e = fwb_launch_status();
     if (e) return e;
     prm.stages = HD == 64 ? 3 : 2;

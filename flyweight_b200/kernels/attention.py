@@ -268,11 +268,24 @@ def paged_attention(ctx, q, cache, block_table, n_heads, window, scale, out_dtyp
 
 
 def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int, own_pages: int, wide: bool):
-    """How the work of ``shared_prefix_attention`` is cut: slices of a group's shared pages, slices of a token's own ones.
-    ``wide``: 128 rows a block and two blocks an SM (the tensor cores), else 64 and one or two."""
+    """How the work of ``shared_prefix_attention`` is cut: slices of a group's shared pages (0: every token walks them by itself,
+    in one launch), slices of a token's own ones.  ``wide``: the tensor cores' kernels (128 rows a block and two blocks an SM), else
+    64 rows."""
+    # Measured on B200 (us, requests of one token and one own page, 16 heads over 8 of 64 / 8 heads over 2 of 128; shared pages
+    # once a group in two launches, and by every token in one): 2 requests, 8 pages 10.0 6.6 / 9.6 7.3, 64 pages 13.8 12.1 / 12.8 12.8,
+    # 128 pages 16.6 18.6 / 14.1 18.7; 16 requests, 16 pages 13.7 11.5 / 11.7 9.4, 64 pages 15.1 28.8 / 14.5 14.7; 64 requests, 8 pages
+    # 14.8 13.5 / 12.8 10.0, 16 pages 16.3 20.7 / 13.5 13.4, 128 pages 23.0 122 / 24.9 57.4.  A block takes 0.7 us a page, so one launch
+    # is faster up to about eight pages of shared keys a block (with up to eight blocks a token and KV head where there are few).
+    pairs = n_tokens * n_kv * -(-group // 16)
+    if wide:
+        own = 1
+        while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and shared_pages + own_pages >= 2 * own:
+            own *= 2
+        if -(-shared_pages // own) * -(-pairs // (4 * SM_COUNT)) <= 8:
+            return 0, own
     row_tiles = -(-n_tokens * group // (128 if wide else 64)) * n_kv
     shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles))
-    own, pairs = 1, n_tokens * n_kv * -(-group // 16)
+    own = 1
     while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and own_pages >= 8 * own:
         own *= 2
     return shared, own
@@ -340,13 +353,16 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     wide = dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
     splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, width if shared_pages is None else min(width, shared_pages),
                                        width if own_pages is None else own_pages, wide)
-    # every slice's maximum and sum, then (on a border of 16 bytes) its O
-    rows = T * n_heads * splits
-    rows += rows & 1
-    scratch = torch.empty(rows * (head_dim + 2), dtype=torch.float32, device=q.device)
-    part_ml = scratch.data_ptr()
+    part_ml = part_o = None
+    if splits:
+        # every slice's maximum and sum, then (on a border of 16 bytes) its O
+        rows = T * n_heads * splits
+        rows += rows & 1
+        scratch = torch.empty(rows * (head_dim + 2), dtype=torch.float32, device=q.device)
+        part_ml = scratch.data_ptr()
+        part_o = part_ml + 8 * rows
     lib.call("fwb_attention_prefix", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), 1 if dtype is torch.bfloat16 else 0,
              positions.data_ptr(), tok_seg.data_ptr(), block_table.data_ptr(), requests, width, num_pages, group_start.data_ptr(),
-             group_pages.data_ptr(), groups, part_ml + 8 * rows, part_ml, out.data_ptr(), T, n_heads, n_kv, head_dim,
-             splits, own, scale, lib.ptr(sink), softcap, lib.stream(), launches=2)
+             group_pages.data_ptr(), groups, part_o, part_ml, out.data_ptr(), T, n_heads, n_kv, head_dim,
+             splits, own, scale, lib.ptr(sink), softcap, lib.stream(), launches=2 if splits else 1)
     return out

@@ -93,6 +93,20 @@ def attend(case, **more):
     return attention.shared_prefix_attention(**{**case.device(), **more})
 
 
+@pytest.fixture(params=["two launches", "one launch"])
+def cut(request, monkeypatch):
+    """The sizes of most tests here choose one launch; the same with the shared pages once a group, in slices."""
+    from flyweight_b200.kernels import attention
+    rule = attention.shared_prefix_splits
+
+    def pinned(n_tokens, n_kv, group, shared, own, wide):
+        if request.param == "one launch" and wide:
+            return 0, 1 if own < 4 else 4
+        return (min(shared, 7), 2 if wide and own > 3 else 1)
+    monkeypatch.setattr(attention, "shared_prefix_splits", pinned)
+    yield rule
+
+
 SHAPES = [(4, 4, 64), (8, 2, 64), (6, 2, 128), (16, 1, 128), (8, 8, 16), (10, 5, 80), (12, 4, 96), (9, 3, 48), (5, 1, 32)]
 WIDE = [(3, 1, 256), (20, 1, 64), (128, 1, 64), (70, 1, 40), (2, 2, 200)]
 BATCHES = {
@@ -109,14 +123,14 @@ BATCHES = {
 @pytest.mark.parametrize("batch", sorted(BATCHES))
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads,kv,dim", SHAPES)
-def test_against_one_softmax_a_token(batch, dtype, heads, kv, dim):
+def test_against_one_softmax_a_token(cut, batch, dtype, heads, kv, dim):
     case = Case(BATCHES[batch], heads, kv, dim, dtype, idle=3 if batch == "groups" else 0)
     case.check(attend(case))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads,kv,dim", WIDE)
-def test_wide_heads_and_wide_groups(dtype, heads, kv, dim):
+def test_wide_heads_and_wide_groups(cut, dtype, heads, kv, dim):
     case = Case(BATCHES["groups"], heads, kv, dim, dtype, idle=1)
     case.check(attend(case))
 
@@ -124,14 +138,14 @@ def test_wide_heads_and_wide_groups(dtype, heads, kv, dim):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 80, 128])
 @pytest.mark.parametrize("sink,softcap", [(True, 0.0), (False, 5.0), (True, 30.0)])
-def test_sink_and_cap(dtype, dim, sink, softcap):
+def test_sink_and_cap(cut, dtype, dim, sink, softcap):
     case = Case(BATCHES["groups"], 8, 2, dim, dtype, sink=sink, softcap=softcap, q_scale=3.0)
     case.check(attend(case))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 96])
-def test_positions_inside_the_shared_pages_and_before_the_first(dtype, dim):
+def test_positions_inside_the_shared_pages_and_before_the_first(cut, dtype, dim):
     """A token may stand inside the shared pages (it sees them up to itself) or nowhere (a padded row)."""
     case = Case([(4, [(1, 10), (1, 10), (1, 10), (1, 10), (1, 10)])], 8, 2, dim, dtype)
     case.positions = [0, 100, 255, -1, 256 + 9]
@@ -140,7 +154,7 @@ def test_positions_inside_the_shared_pages_and_before_the_first(dtype, dim):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128, 80])
-def test_what_lies_behind_the_last_key_is_not_seen(dtype, dim):
+def test_what_lies_behind_the_last_key_is_not_seen(cut, dtype, dim):
     """Infinities and NaN in keys and values that no token may see: behind the requests' last keys and in unmapped pages."""
     case = Case([(2, [(1, 5), (1, 70)]), (0, [(1, 33)])], 8, 4, dim, dtype)
     want = attend(case).clone()
@@ -156,7 +170,7 @@ def test_what_lies_behind_the_last_key_is_not_seen(dtype, dim):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128, 80])
-def test_the_lowest_and_largest_numbers(dtype, dim):
+def test_the_lowest_and_largest_numbers(cut, dtype, dim):
     """Scores far apart between shared and own keys, either way round: the part that weighs nothing adds nothing."""
     for which in (0, 1):
         case = Case([(3, [(1, 70), (1, 3)])], 4, 2, dim, dtype)
@@ -176,7 +190,7 @@ def test_the_cut_of_the_work_is_only_a_cut(dtype):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-def test_equals_the_attention_that_reads_every_request(dim):
+def test_equals_the_attention_that_reads_every_request(cut, dim):
     """Beside the framework's own decode attention on the same pages: two bfloat16 computations of one value."""
     from flyweight_b200.kernels import attention, ops
     case = Case([(20, [(1, 33 * i + 1) for i in range(9)])], 16, 4, dim, torch.bfloat16)
@@ -188,7 +202,7 @@ def test_equals_the_attention_that_reads_every_request(dim):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_pages_outside_the_pool_are_not_read(dtype):
+def test_pages_outside_the_pool_are_not_read(cut, dtype):
     """A page id that is none: its keys are not seen, and nothing is read for it."""
     for dim in (64, 80):
         case = Case([(3, [(1, 10), (1, 100)])], 4, 2, dim, dtype)
@@ -202,6 +216,20 @@ def test_pages_outside_the_pool_are_not_read(dtype):
         short.rows = [[r[0], r[2], r[3]] if i == 0 else [r[0], r[2], r[4]] for i, r in enumerate(short.rows)]
         short.positions = [2 * PAGE + 9, 2 * PAGE + 35]
         short.check(got)
+
+
+def test_the_rule_of_the_cut():
+    """Few shared pages a block: one launch; else as many slices as fill the SMs twice, at most 64 and one a page."""
+    from flyweight_b200.kernels import attention
+    rule = attention.shared_prefix_splits
+    assert rule(2, 8, 2, 7, 1, True) == (0, 8) and rule(2, 8, 2, 128, 1, True) == (296 // 8, 1)
+    assert rule(64, 8, 4, 8, 1, True)[0] == 0 and rule(64, 8, 4, 16, 1, True)[0] == 16
+    assert rule(2048, 8, 4, 8, 1, True)[0] > 0            # several rounds of blocks
+    assert rule(2, 8, 2, 7, 1, False) == (7, 1)           # the 32-bit kernels always read the shared pages once
+    for tokens in (1, 5, 300):
+        for pages in (1, 9, 1000):
+            shared, own = rule(tokens, 4, 6, pages, 50, True)
+            assert 0 <= shared <= min(64, pages) and own in (1, 2, 4, 8)
 
 
 def test_no_groups_and_no_tokens():
