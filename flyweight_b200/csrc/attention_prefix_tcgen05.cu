@@ -470,7 +470,7 @@ struct OwnLayout {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(OWN_THREADS, HD == 64 ? 4 : 2)
+__global__ void __launch_bounds__(OWN_THREADS, HD == 64 ? 4 : 3)
 own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params prm) {
     using L = OwnLayout<HD>;
     constexpr int MAX_STAGES = 8;

@@ -680,11 +680,23 @@ FWB_API int fwb_rows_int8(const void* x, int x_bf16, const float* delta, const f
                           float* scales, int R, int K, int stride, float eps, cudaStream_t stream);
 
 // The same for rows that are no integers yet: x [M][K] bf16 (x_bf16) or fp32; scratch: M * stride bytes for the integers and
-// 4 M behind them for the scales, stride = K rounded up to 16.
+// 4 M behind them for the scales, stride = K rounded up to 16.  Without scratch (null): in one launch, for at most 8 tokens and 4,096
+// columns, K a multiple of 8 and the rows on borders of 16 bytes.
 FWB_API int fwb_linear_int8(const void* x, int x_bf16, void* scratch, const void* W, const float* ws, void* Y, const float* addend,
                             int M, int N, int K, int w_stride, int w_rows, int epilogue, int up_row_offset, float gate_limit,
                             cudaStream_t stream) {
     const int stride = (K + 15) & ~15;
+    if (!scratch) {
+        const int code = epilogue & 0xff;
+        if (M <= 0 || N <= 0) return FWB_OK;
+        if (!x || !W || !ws || !Y || K <= 0 || w_stride < K) return FWB_BAD_ARGUMENT;
+        if ((w_stride & 15) || ((uintptr_t)W & 15)) return FWB_UNSUPPORTED;
+        if (code == EPI_ADD_F32 && !addend) return FWB_BAD_ARGUMENT;
+        if (code == EPI_GATED_BF16 ? (up_row_offset < N || w_rows < up_row_offset + N) : w_rows < N) return FWB_BAD_ARGUMENT;
+        const Product p{nullptr, (const signed char*)W, nullptr, ws, Y, addend, M, N, K, stride, w_stride, w_rows,
+                        up_row_offset, epilogue >> 8, gate_limit, status_word()};
+        return few_raw_tokens(p, x, x_bf16 != 0, code, stream);
+    }
     float* scales = reinterpret_cast<float*>(static_cast<char*>(scratch) + (size_t)M * stride);
     const int status = fwb_rows_int8(x, x_bf16, nullptr, nullptr, nullptr, scratch, scales, M, K, stride, 0.0f, stream);
     if (status != FWB_OK) return status;

@@ -39,6 +39,10 @@ __device__ __forceinline__ void store(const Product& p, size_t at, float v, floa
 // The product of a few tokens (host function, linear_rows_int8.cu); at most MAX_FEW of them.
 constexpr int MAX_FEW = 32;
 int few_tokens(const Product& p, int epilogue, cudaStream_t stream);
+// The same on rows that are no integers yet (raw: [M][K], rows on borders of 16 bytes), which every block brings to integers by
+// itself: for at most MAX_RAW tokens and MAX_RAW_K columns, K a multiple of 8.
+constexpr int MAX_RAW = 8, MAX_RAW_K = 4096;
+int few_raw_tokens(const Product& p, const void* raw, bool is_bf16, int epilogue, cudaStream_t stream);
 
 }  // namespace int8
 }  // namespace fwb

@@ -3,9 +3,7 @@
 //   s_r = max_k |y_rk| / 127      q_rk = round(y_rk / s_r), ties to even
 //
 // with y the rows themselves or their RMS norm, y = (x r) w, r = 1 / sqrt(mean(x^2) + eps), behind a residual sum
-// x += delta where there is one.  The quotient's rounding is the exact one: a product with 1 / s decides all but the values
-// next to a half (it is off by 127 * 2^-23 at most), and there the remainder decides.  A row of zeros has the scale 0.  A row that holds an infinity or a NaN has the scale NaN:
-// whatever is made of it is NaN.
+// x += delta where there is one (int8_quantize.cuh: the rounding, rows of zeros, infinities).
 //
 // Rows of integers lie `stride` bytes apart, a multiple of 16 (what TMA asks of a row), and are zero behind column K.
 //
@@ -13,15 +11,14 @@
 // Many rows: a warp has up to 2,048 columns of one, so that as much as possible is on the way at once and nobody waits at
 // a barrier; few: a block has a row, a thread eight columns, for the shortest way through.  Rounding by adding 1.5 * 2^23, whose
 // low byte is the integer: the conversion instructions have a quarter of the adders' rate.
-#include "common.cuh"
+#include "int8_quantize.cuh"
 
 using namespace fwb;
+using namespace fwb::int8;
 
 namespace {
 
-constexpr int CHUNK = 8;                 // elements a thread takes at once
 constexpr int WARP_ROWS = 4;             // warps of a block whose warps have a row each
-constexpr float TINY_ROW = 1e-30f;       // a row without a larger value is taken as zeros: its scale would be no normal number
 
 struct RowsInt8Params {
     const void* x;               // [.][K] bf16 or fp32
@@ -69,39 +66,6 @@ __device__ __forceinline__ void values(const Raw<__nv_bfloat16>& r, float (&v)[C
         v[2 * i] = __uint_as_float(p[i] << 16);
         v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
     }
-}
-
-// Eight values' integers.
-//
-// Checked: n = x (1 / s) rounded is the integer or its neighbour; e = x - n s has no rounding error (a multiple of the smaller
-// of x's and s's last places, and at most about s / 2), so |e| against s / 2 tells.
-//
-// Not checked, for values of eight bits under a maximum m of eight bits (bfloat16 rows): 254 |x| / m is an odd integer, and x / (m / 127)
-// a tie, or it is 2^-8 or more away from one.  s is m / 127 rounded, so the ties all lie on one side of their halves, by 2^-24 of
-// themselves at most; `inv` is 1 / s moved by 2^-22 of itself towards that side, which decides every tie and nothing else.
-template <bool CHECKED>
-__device__ __forceinline__ uint2 quantize(const float (&v)[CHUNK], float s, float inv) {
-    constexpr float ROUND = 12582912.0f;               // 1.5 * 2^23
-    uint32_t word[CHUNK];
-    float off = 0.0f;
-#pragma unroll
-    for (int i = 0; i < CHUNK; ++i) {
-        const float n = fmaf(v[i], inv, ROUND);
-        word[i] = __float_as_uint(n);
-        if (CHECKED) off = fmaxf(off, fabsf(fmaf(-__fsub_rn(n, ROUND), s, v[i])));
-    }
-    const float half = 0.5f * s;
-    if (CHECKED && off >= half) {
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const float n = __uint_as_float(word[i]), e = fmaf(-__fsub_rn(n, ROUND), s, v[i]);
-            if (fabsf(e) > half || (fabsf(e) == half && (word[i] & 1))) word[i] += e > 0.0f ? 1 : -1;
-        }
-    }
-    uint2 packed;
-    packed.x = __byte_perm(__byte_perm(word[0], word[1], 0x0040), __byte_perm(word[2], word[3], 0x0040), 0x5410);
-    packed.y = __byte_perm(__byte_perm(word[4], word[5], 0x0040), __byte_perm(word[6], word[7], 0x0040), 0x5410);
-    return packed;
 }
 
 // What the threads of a row hold, put together; every one of them gets the result.
@@ -211,19 +175,12 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : CHUNKS == 8 ? 256 : 10
             if (FORM == PLAIN || prm.vector || k + i < K) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     });
     top = row_max<WARP>(top, tops);
-    const float most = __uint_as_float(top), s = most / 127.0f;
-    const bool finite = top < 0x7f800000u, zero = most < TINY_ROW;
-    float inv = !finite || zero ? 0.0f : 1.0f / s;
-    // which side of its half a tie of a bfloat16 row lies on: s above m / 127, towards zero; s below, away from it
-    const float above = fmaf(s, 127.0f, -most);
-    const bool sided = sizeof(T) == 2 && above != 0.0f;
-    if (sided) inv = fmaf(inv, above > 0.0f ? -0x1p-22f : 0x1p-22f, inv);
-    if (k0 == 0) prm.scales[r] = !finite ? __int_as_float(0x7fffffff) : zero ? 0.0f : s;
+    const RowScale scale = row_scale(top, sizeof(T) == 2);
+    if (k0 == 0) prm.scales[r] = scale.stored;
     signed char* out = prm.q + (size_t)r * prm.stride;
     each([&](int k, float (&v)[CHUNK]) {
         if (FORM != PLAIN && CHUNKS == 0) finish_norm(k, v);
-        uint2 packed = sided ? quantize<false>(v, s, inv) : quantize<true>(v, s, inv);
-        if (inv == 0.0f) packed = make_uint2(0, 0);
+        uint2 packed = quantize(v, scale);
         if (FORM != PLAIN && !prm.vector && k + CHUNK > K) {           // what a norm made of columns that are none
             const unsigned long long mask = ~0ull >> (8 * (k + CHUNK - K));
             packed.x &= (uint32_t)mask, packed.y &= (uint32_t)(mask >> 32);

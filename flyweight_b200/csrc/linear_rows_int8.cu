@@ -8,9 +8,13 @@
 //     moment on: nothing in the stream writes weights.  Two CTAs an SM, or four small ones.
 //   * mma.sync of 16 tokens x 8 features x 32 k on 8-bit integers; a lane's 16-byte read is sixteen k of one feature, and the k
 //     of a block are dealt to the fragments' slots in that order for both operands.
+//   * Rows that are no integers yet (at most eight): a first pass over them finds the rows' largest magnitudes, then every block makes
+//     the integers of the k that a lane feeds to its products, where int8_rows.cu would make them in a launch of its own.  The
+//     same integers: a product's bits do not depend on it.
 //   * The warps' sums meet in shared memory; integers, so their order is of no consequence.
 // Every wait on an mbarrier is bounded as in the tcgen05 products.
 #include "int8_product.cuh"
+#include "int8_quantize.cuh"
 
 using namespace fwb;
 using namespace fwb::tc5;
@@ -21,18 +25,41 @@ namespace {
 constexpr int SMEM_OF_SM = 224 * 1024;
 constexpr int MAX_SLOTS = 8;
 constexpr long ALL_CTAS_FROM = 2 << 20;
+constexpr int EIGHT = fwb::int8::CHUNK;
 
 struct RowsParams {
     Product p;
     int Kp;                      // bytes of a row that hold k: K rounded up to 16
     int units;                   // groups of eight features of one half per CTA
     int slots;                   // depth of the ring
+    const void* raw;             // RAW: [M][K] rows that are no integers yet
 };
+
+enum Raw : int { INTEGERS = 0, RAW_BF16 = 1, RAW_F32 = 2 };
+
+// Eight values of a raw row from column k on, zeros from K on (K and k are multiples of 8).
+template <int RAW>
+__device__ __forceinline__ void raw_values(const RowsParams& prm, int row, int k, float (&v)[EIGHT]);
 
 __device__ __forceinline__ uint4 load_rows(const void* at) {     // written by the kernel before: not .nc
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at) : "memory");
     return v;
+}
+template <>
+__device__ __forceinline__ void raw_values<RAW_BF16>(const RowsParams& prm, int row, int k, float (&v)[EIGHT]) {
+    const uint4 a = k < prm.p.K ? load_rows(static_cast<const __nv_bfloat16*>(prm.raw) + (size_t)row * prm.p.K + k) : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void raw_values<RAW_F32>(const RowsParams& prm, int row, int k, float (&v)[EIGHT]) {
+    const float* at = static_cast<const float*>(prm.raw) + (size_t)row * prm.p.K + k;
+    const uint4 none = make_uint4(0, 0, 0, 0), a = k < prm.p.K ? load_rows(at) : none, b = k < prm.p.K ? load_rows(at + 4) : none;
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
 }
 __device__ __forceinline__ void mma_16x8x32(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -44,7 +71,7 @@ __device__ __forceinline__ void mma_16x8x32(int (&d)[4], uint32_t a0, uint32_t a
 __host__ __device__ constexpr int row_stride(int bytes) { return ((bytes + 127) & ~127) + 64; }
 
 // WARPS that sum, CTAS an SM, R8 groups of eight token rows, KBLK blocks of 64 k a warp takes in a step.
-template <int WARPS, int CTAS, int R8, int KBLK, int EPI>
+template <int WARPS, int CTAS, int R8, int KBLK, int EPI, int RAW>
 __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kernel(const RowsParams prm) {
     constexpr int NACC = EPI == EPI_GATED_BF16 ? 2 : 1, THREADS = 32 * (WARPS + 1);
     constexpr int MT = (R8 + 1) / 2;                   // 16-row tiles of the product
@@ -52,6 +79,7 @@ __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kerne
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full_bar[MAX_SLOTS], empty_bar[MAX_SLOTS];
     __shared__ int abort_word;
+    __shared__ unsigned tops[MAX_RAW];                 // RAW: the rows' largest magnitudes, as bits
     volatile int* abort_flag = &abort_word;
     const Product& p = prm.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -70,6 +98,7 @@ __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kerne
             mbar_init(&empty_bar[s], WARPS);
         }
         abort_word = 0;
+        for (int r = 0; r < MAX_RAW; ++r) tops[r] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -101,16 +130,50 @@ __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kerne
 
     if (warp < WARPS) {
         // ---- activations
+        RowScale scale{};
+        if constexpr (RAW != INTEGERS) {
+            // as many warps a row as there are, each with a share of its eights (or several rows a warp)
+            const int parts = p.M < WARPS ? WARPS / p.M : 1, part = p.M < WARPS ? warp / p.M : 0;
+            for (int row = p.M < WARPS ? warp % p.M : warp; row < p.M && part < parts; row += WARPS) {
+                unsigned top = 0;
+#pragma unroll 4
+                for (int k = (part * 32 + lane) * EIGHT; k < p.K; k += parts * 32 * EIGHT) {
+                    float v[EIGHT];
+                    raw_values<RAW>(prm, row, k, v);
+#pragma unroll
+                    for (int i = 0; i < EIGHT; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) atomicMax(&tops[row], top);
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+            scale = row_scale(tops[g < p.M ? g : 0], RAW == RAW_BF16);
+        }
         uint4 x_next[KBLK][R8];
         const signed char* x_at[R8];
 #pragma unroll
         for (int r = 0; r < R8; ++r) x_at[r] = g + 8 * r < p.M ? p.x + (size_t)(g + 8 * r) * p.x_stride : nullptr;
         auto fetch_rows = [&](int k) {
+            if constexpr (RAW != INTEGERS) {
 #pragma unroll
-            for (int b = 0; b < KBLK; ++b)
+                for (int b = 0; b < KBLK; ++b) {
+                    uint2 one = make_uint2(0, 0), two = make_uint2(0, 0);
+                    if (g < p.M && k + b * 64 < p.K) {
+                        float v[EIGHT];
+                        raw_values<RAW>(prm, g, k + b * 64, v);
+                        one = quantize(v, scale);
+                        raw_values<RAW>(prm, g, k + b * 64 + EIGHT, v);
+                        two = quantize(v, scale);
+                    }
+                    x_next[b][0] = make_uint4(one.x, one.y, two.x, two.y);
+                }
+            } else {
 #pragma unroll
-                for (int r = 0; r < R8; ++r)
-                    x_next[b][r] = x_at[r] && k + b * 64 < Kp ? load_rows(x_at[r] + k + b * 64) : make_uint4(0, 0, 0, 0);
+                for (int b = 0; b < KBLK; ++b)
+#pragma unroll
+                    for (int r = 0; r < R8; ++r)
+                        x_next[b][r] = x_at[r] && k + b * 64 < Kp ? load_rows(x_at[r] + k + b * 64) : make_uint4(0, 0, 0, 0);
+            }
         };
         int x_k = warp * KBLK * 64 + t * 16;
         fetch_rows(x_k);
@@ -180,6 +243,11 @@ __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kerne
 
     // ---- the warps' sums together, and what the caller wants done with them
     const int width = units * 8;
+    if constexpr (RAW != INTEGERS) {
+        // (the maxima become the scales)
+        if (threadIdx.x < MAX_RAW) tops[threadIdx.x] = __float_as_uint(row_scale(tops[threadIdx.x], RAW == RAW_BF16).stored);
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < width * p.M; i += THREADS) {
         const int row = i / width, n = i - row * width, f = unit0 * 8 + n;
         if (f >= p.N) continue;
@@ -192,13 +260,13 @@ __global__ void __launch_bounds__(32 * (WARPS + 1), CTAS) linear_rows_int8_kerne
             int sum = 0;
 #pragma unroll
             for (int wp = 0; wp < WARPS; ++wp) sum += from[(size_t)wp * prm.units * NACC * R8 * 64];
-            value[a] = scaled(sum, p.xs[row], p.ws[a * p.up_row_offset + f]);
+            value[a] = scaled(sum, RAW != INTEGERS ? __uint_as_float(tops[row]) : p.xs[row], p.ws[a * p.up_row_offset + f]);
         }
         store<EPI>(p, at, value[0], value[NACC - 1], add);
     }
 }
 
-template <int WARPS, int CTAS, int R8, int KBLK, int EPI>
+template <int WARPS, int CTAS, int R8, int KBLK, int EPI, int RAW = INTEGERS>
 int launch(RowsParams prm, cudaStream_t stream) {
     constexpr int NACC = EPI == EPI_GATED_BF16 ? 2 : 1, CHUNK = WARPS * KBLK * 64, SLOT = 8 * row_stride(CHUNK);
     constexpr int MOST = 16 / (NACC * R8) ? 16 / (NACC * R8) : 1;    // units a CTA keeps partial sums of: 32 KiB
@@ -216,7 +284,7 @@ int launch(RowsParams prm, cudaStream_t stream) {
     slots = slots > MAX_SLOTS ? MAX_SLOTS : slots;
     slots = slots > steps ? steps : slots;
     prm.slots = slots < 2 ? 2 : slots;
-    auto kernel = linear_rows_int8_kernel<WARPS, CTAS, R8, KBLK, EPI>;
+    auto kernel = linear_rows_int8_kernel<WARPS, CTAS, R8, KBLK, EPI, RAW>;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
@@ -243,12 +311,34 @@ int launch_rows(const RowsParams& prm, cudaStream_t stream) {
 
 int fwb::int8::few_tokens(const Product& p, int epilogue, cudaStream_t stream) {
     if (p.M > MAX_FEW) return FWB_TOO_LARGE;
-    const RowsParams prm{p, (p.K + 15) & ~15, 0, 0};
+    const RowsParams prm{p, (p.K + 15) & ~15, 0, 0, nullptr};
     switch (epilogue) {
         case EPI_F32: return launch_rows<EPI_F32>(prm, stream);
         case EPI_BF16: return launch_rows<EPI_BF16>(prm, stream);
         case EPI_ADD_F32: return launch_rows<EPI_ADD_F32>(prm, stream);
         case EPI_GATED_BF16: return launch_rows<EPI_GATED_BF16>(prm, stream);
+        default: return FWB_UNSUPPORTED;
+    }
+}
+
+namespace {
+template <int EPI>
+int launch_raw(const RowsParams& prm, bool is_bf16, cudaStream_t stream) {
+    const bool is_short = prm.Kp <= SHORT_K;
+    if (is_bf16) return is_short ? launch<4, 4, 1, 4, EPI, RAW_BF16>(prm, stream) : launch<8, 2, 1, 4, EPI, RAW_BF16>(prm, stream);
+    return is_short ? launch<4, 4, 1, 4, EPI, RAW_F32>(prm, stream) : launch<8, 2, 1, 4, EPI, RAW_F32>(prm, stream);
+}
+}  // namespace
+
+int fwb::int8::few_raw_tokens(const Product& p, const void* raw, bool is_bf16, int epilogue, cudaStream_t stream) {
+    if (p.M > MAX_RAW || p.K > MAX_RAW_K) return FWB_TOO_LARGE;
+    if ((p.K & 7) || ((uintptr_t)raw & 15)) return FWB_UNSUPPORTED;
+    const RowsParams prm{p, (p.K + 15) & ~15, 0, 0, raw};
+    switch (epilogue) {
+        case EPI_F32: return launch_raw<EPI_F32>(prm, is_bf16, stream);
+        case EPI_BF16: return launch_raw<EPI_BF16>(prm, is_bf16, stream);
+        case EPI_ADD_F32: return launch_raw<EPI_ADD_F32>(prm, is_bf16, stream);
+        case EPI_GATED_BF16: return launch_raw<EPI_GATED_BF16>(prm, is_bf16, stream);
         default: return FWB_UNSUPPORTED;
     }
 }

@@ -13,6 +13,8 @@
     python -m flyweight_b200.kernels.microbench latent-decode --batch 64 --context 4096
     python -m flyweight_b200.kernels.microbench latent-prefill --tokens 2048
     python -m flyweight_b200.kernels.microbench sample --rows 8 --top-k 40
+    python -m flyweight_b200.kernels.microbench int8-linear --tokens 64 --features 2048 --k 8192 [--gated]
+    python -m flyweight_b200.kernels.microbench shared-prefix --batch 64 --prefix 8192 --own 500
 
 It is what the ncu summaries under ``profiles/`` were captured from (small cases of the same
 kernels the engine runs), and a quick way to see what a shape costs.  Weight matrices are
@@ -454,6 +456,49 @@ def run_sample(args) -> dict:
             "kernel_only": bool(args.kernel_only), "us": us, "gb_s": rows * vocab * 4 / us / 1e3}
 
 
+def run_int8_linear(args) -> dict:
+    """Rows to integers and the 8-bit product behind them (with --gated gate and up projection), bfloat16 rows."""
+    from . import int8
+    M, N, K = args.tokens, args.features, args.k
+    rows = 2 * N if args.gated else N
+    copies = max(2, min(32, (300 << 20) // (rows * K)))
+    weights = [int8.matrix_int8(torch.randn(rows, K, device="cuda").to(torch.bfloat16)) for _ in range(copies)]
+    x = torch.randn(M, K, device="cuda").to(torch.bfloat16)
+
+    def steps():
+        for w in weights:
+            int8.gated_int8(x, w) if args.gated else int8.linear_int8(x, w, torch.float32)
+    us = _time_graph(steps, max(1, args.repeat // copies)) / copies
+    ops = 2.0 * M * rows * K
+    return {"kernel": "int8-linear", "tokens": M, "features": N, "k": K, "gated": args.gated, "us": us,
+            "tops": ops / us / 1e6, "weight_gbs": rows * K / us / 1e3}
+
+
+def run_shared_prefix(args) -> dict:
+    """Attention of one token of every request behind one shared prefix and up to --own keys of its own."""
+    from .attention import shared_prefix_attention
+    pages, own = max(1, args.prefix // 64), [max(1, args.own - (r * 37) % args.own) for r in range(args.batch)]
+    most = -(-max(own) // 64)
+    total = pages + args.batch * most
+    dtype = torch.float32 if args.fp32 else torch.bfloat16
+    pool = (total, args.kv_heads, 64, args.head_dim)
+    k, v = (torch.randn(pool, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn(args.batch, args.heads * args.head_dim, device="cuda").to(dtype)
+
+    def i32(values):
+        return torch.tensor(values, dtype=torch.int32, device="cuda")
+    table = i32([list(range(pages)) + [pages + r * most + i for i in range(most)] for r in range(args.batch)])
+    positions, segment = i32([pages * 64 + n - 1 for n in own]), i32(list(range(args.batch)))
+    starts, shared = i32([0, args.batch]), i32([pages])
+    out = torch.empty_like(q)
+    us = _time_graph(lambda: shared_prefix_attention(q, k, v, positions, segment, table, starts, shared, args.heads,
+                                                     args.head_dim ** -0.5, out=out, shared_pages=pages, own_pages=most), args.repeat)
+    keys = 64 * pages + sum(own)
+    return {"kernel": "shared-prefix", "batch": args.batch, "prefix": 64 * pages, "us": us,
+            "gbs": 2.0 * keys * args.kv_heads * args.head_dim * q.element_size() / us / 1e3,
+            "tflops": 4.0 * args.heads * args.head_dim * (64 * pages * args.batch + sum(own)) / us / 1e6}
+
+
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(prog="python -m flyweight_b200.kernels.microbench",
                                      description=__doc__,
@@ -561,6 +606,19 @@ def main(argv=None) -> int:
     smp.add_argument("--top-p", type=float, default=0.95)
     smp.add_argument("--logit-scale", type=float, default=3.0, help="spread of the Gaussian logits")
     smp.add_argument("--kernel-only", action="store_true", help="time the launches without the Python call around them")
+    i8 = sub.add_parser("int8-linear")
+    i8.add_argument("--tokens", type=int, default=64)
+    i8.add_argument("--features", type=int, default=2048)
+    i8.add_argument("--k", type=int, default=8192)
+    i8.add_argument("--gated", action="store_true", help="gate and up projection of that many features each")
+    pre = sub.add_parser("shared-prefix")
+    pre.add_argument("--batch", type=int, default=64)
+    pre.add_argument("--prefix", type=int, default=8192)
+    pre.add_argument("--own", type=int, default=500)
+    pre.add_argument("--heads", type=int, default=32)
+    pre.add_argument("--kv-heads", type=int, default=8)
+    pre.add_argument("--head-dim", type=int, default=64)
+    pre.add_argument("--fp32", action="store_true")
     for p in sub.choices.values():
         p.add_argument("--repeat", type=int, default=20)
     args = parser.parse_args(argv)
@@ -569,7 +627,8 @@ def main(argv=None) -> int:
               "causal-conv": run_causal_conv,
               "qk-norm-rope": run_qk_norm_rope, "sample": run_sample, "delta-rule": run_delta_rule,
               "linear-attention": run_linear_attention, "gated-average": run_gated_average, "route": run_route,
-              "state-space": run_state_space, "latent-decode": run_latent_decode, "latent-prefill": run_latent_prefill}[args.kernel]
+              "state-space": run_state_space, "latent-decode": run_latent_decode, "latent-prefill": run_latent_prefill,
+              "int8-linear": run_int8_linear, "shared-prefix": run_shared_prefix}[args.kernel]
     print(json.dumps(runner(args)))
     return 0
 

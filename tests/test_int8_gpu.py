@@ -235,6 +235,36 @@ def test_the_largest_integers_do_not_overflow():
     assert ((got.to(F64)[0] - want).abs() <= want * 4 * HALF).all() and torch.equal(got[1], -got[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(1, 8, 3), (1, 2048, 300), (2, 1032, 65), (3, 4096, 100), (5, 24, 1000), (7, 2040, 17), (8, 4088, 260),
+                                   (8, 512, 2400), (1, 1024, 4000)])
+def test_a_few_rows_become_integers_inside_the_product(M, K, N, dtype):
+    """One launch for at most eight rows: the bits of two, with every epilogue, with rows of zeros, infinities and NaN."""
+    from flyweight_b200.kernels import int8
+    from flyweight_b200.kernels.lib import launch_count
+    x = rows_of(M, K, dtype)
+    if M > 4:
+        x[1], x[2, 0], x[3, K - 1] = 0, math.nan, math.inf
+    x, matrix = x.to(DEV), int8.matrix_int8(rows_of(2 * N, K, torch.bfloat16, 1).to(DEV))
+    rows, addend = int8.rows_int8(x), torch.randn(M, 2 * N, device=DEV)
+    for call in (lambda a: int8.linear_int8(a, matrix, torch.float32), lambda a: int8.linear_int8(a, matrix, torch.bfloat16),
+                 lambda a: int8.linear_int8(a, matrix, torch.float32, addend=addend), lambda a: int8.gated_int8(a, matrix, "relu")):
+        two, before = call(rows), launch_count()
+        one = call(x)
+        assert launch_count() - before == 1
+        assert torch.equal(torch.isnan(one), torch.isnan(two)) and torch.equal(one.nan_to_num(0), two.nan_to_num(0))
+
+
+def test_rows_off_a_border_take_two_launches():
+    from flyweight_b200.kernels import int8
+    matrix = int8.matrix_int8(rows_of(50, 64, torch.bfloat16, 1).to(DEV))
+    held = rows_of(1, 1 + 3 * 64, torch.bfloat16).to(DEV).flatten()
+    off = held[1:].view(3, 64)
+    assert off.data_ptr() % 16 and off.is_contiguous()
+    assert torch.equal(int8.linear_int8(off, matrix, torch.float32), int8.linear_int8(off.clone(), matrix, torch.float32))
+    assert torch.equal(int8.rows_int8(off).values, int8.rows_int8(off.clone()).values)
+
+
 def test_inputs_in_32_bits_are_brought_to_integers_first():
     from flyweight_b200.kernels import int8
     for M in (1, 6, 130):
