@@ -267,7 +267,7 @@ def paged_attention(ctx, q, cache, block_table, n_heads, window, scale, out_dtyp
                               keep_first=keep_first)
 
 
-def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int, own_pages: int, wide: bool):
+def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int, own_pages: int, wide: bool, groups: int = 1):
     """How the work of ``shared_prefix_attention`` is cut: slices of a group's shared pages (0: every token walks them by itself,
     in one launch), slices of a token's own ones.  ``wide``: the tensor cores' kernels (128 rows a block and two blocks an SM), else
     64 rows."""
@@ -283,7 +283,10 @@ def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int
             own *= 2
         if -(-shared_pages // own) * -(-pairs // (4 * SM_COUNT)) <= 8:
             return 0, own
-    row_tiles = -(-n_tokens * group // (128 if wide else 64)) * n_kv
+    # the tiles of a group are its own: half a tile more for every further group (53 requests of three tokens in six groups, 24 heads over 4
+    # of 128: counted without, 312 blocks ran in two rounds, 62.8 us; with, 58.3)
+    chunk = min(group, 128 if wide else 64)
+    row_tiles = (-(-n_tokens // ((128 if wide else 64) // chunk)) + (groups - 1) // 2) * -(-group // chunk) * n_kv
     shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles))
     own = 1
     while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and own_pages >= 8 * own:
@@ -352,7 +355,7 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
         return out
     wide = dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
     splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, width if shared_pages is None else min(width, shared_pages),
-                                       width if own_pages is None else own_pages, wide)
+                                       width if own_pages is None else own_pages, wide, groups)
     part_ml = part_o = None
     if splits:
         # every slice's maximum and sum, then (on a border of 16 bytes) its O

@@ -99,7 +99,7 @@ def cut(request, monkeypatch):
     from flyweight_b200.kernels import attention
     rule = attention.shared_prefix_splits
 
-    def pinned(n_tokens, n_kv, group, shared, own, wide):
+    def pinned(n_tokens, n_kv, group, shared, own, wide, groups):
         if request.param == "one launch" and wide:
             return 0, 1 if own < 4 else 4
         return (min(shared, 7), 2 if wide and own > 3 else 1)
