@@ -9,6 +9,8 @@ Everything else (the 32-bit path, head sizes above 128) runs the SIMT kernel.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import lib, ops
@@ -267,7 +269,8 @@ def paged_attention(ctx, q, cache, block_table, n_heads, window, scale, out_dtyp
                               keep_first=keep_first)
 
 
-def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int, own_pages: int, wide: bool, groups: int = 1):
+def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, head_dim: int, shared_pages: int, own_pages: int, wide: bool,
+                         groups: int = 1):
     """How the work of ``shared_prefix_attention`` is cut: slices of a group's shared pages (0: every token walks them by itself,
     in one launch), slices of a token's own ones.  ``wide``: the tensor cores' kernels (128 rows a block and two blocks an SM), else
     64 rows."""
@@ -283,11 +286,19 @@ def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, shared_pages: int
             own *= 2
         if -(-shared_pages // own) * -(-pairs // (4 * SM_COUNT)) <= 8:
             return 0, own
-    # the tiles of a group are its own: half a tile more for every further group (53 requests of three tokens in six groups, 24 heads over 4
-    # of 128: counted without, 312 blocks ran in two rounds, 62.8 us; with, 58.3)
-    chunk = min(group, 128 if wide else 64)
-    row_tiles = (-(-n_tokens // ((128 if wide else 64) // chunk)) + (groups - 1) // 2) * -(-group // chunk) * n_kv
-    shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles))
+    # A slice's walk takes 0.63 us a page (1.1 at head sizes above 64, 2 in fp32), and its results 1 us a megabyte, there and back:
+    # 64 requests, 8 heads over 2 of 128, 128 pages in 8 16 32 64 slices 30.7 22.4 20.2 27.0; 2 requests, 16 heads over 8 of 64, 512 pages
+    # in 8 16 32 64 slices 52.1 32.0 27.2 33.2.  Not more blocks than the SMs hold at once; the tiles of a group are its own, half a
+    # tile more for every further group (53 requests of three tokens in six groups, counted without: two rounds, 62.8; with, 58.3).
+    rows = 128 if wide else 64
+    chunk = min(group, rows)
+    row_tiles = (-(-n_tokens // (rows // chunk)) + (groups - 1) // 2) * -(-group // chunk) * n_kv
+    page_us = 2.0 if not wide else 0.63 if head_dim <= 64 else 1.1
+    best = math.sqrt(page_us * shared_pages / (4e-6 * n_tokens * n_kv * group * head_dim))
+    shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles, round(best)))
+    if wide and head_dim <= 64:
+        per = -(-shared_pages // shared)
+        shared = -(-shared_pages // (per + (per & 1)))         # steps of two pages
     own = 1
     while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and own_pages >= 8 * own:
         own *= 2
@@ -354,7 +365,7 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     if T == 0 or groups == 0:
         return out
     wide = dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
-    splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, width if shared_pages is None else min(width, shared_pages),
+    splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, head_dim, width if shared_pages is None else min(width, shared_pages),
                                        width if own_pages is None else own_pages, wide, groups)
     part_ml = part_o = None
     if splits:

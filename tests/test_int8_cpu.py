@@ -42,7 +42,7 @@ def test_the_rows_say_their_layout():
 def test_the_cut_of_the_shared_pages(tokens, pages):
     from flyweight_b200.kernels.attention import shared_prefix_splits
     for wide in (False, True):
-        shared, own = shared_prefix_splits(tokens, 8, 4, pages, 3, wide)
+        shared, own = shared_prefix_splits(tokens, 8, 4, 64, pages, 3, wide)
         assert own in (1, 2, 4, 8) and 0 <= shared <= min(64, pages) and (shared > 0 or wide)
         # never more blocks than fill the SMs twice over, but for the one slice that there always is
         assert shared <= 1 or shared * 8 * -(-tokens * 4 // (128 if wide else 64)) <= 2 * 148

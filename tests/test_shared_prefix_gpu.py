@@ -99,7 +99,7 @@ def cut(request, monkeypatch):
     from flyweight_b200.kernels import attention
     rule = attention.shared_prefix_splits
 
-    def pinned(n_tokens, n_kv, group, shared, own, wide, groups):
+    def pinned(n_tokens, n_kv, group, head_dim, shared, own, wide, groups):
         if request.param == "one launch" and wide:
             return 0, 1 if own < 4 else 4
         return (min(shared, 7), 2 if wide and own > 3 else 1)
@@ -219,16 +219,18 @@ def test_pages_outside_the_pool_are_not_read(cut, dtype):
 
 
 def test_the_rule_of_the_cut():
-    """Few shared pages a block: one launch; else as many slices as fill the SMs twice, at most 64 and one a page."""
+    """Few shared pages a block: one launch; else slices by what walking a page and what a slice's results cost, not more than fill
+    the SMs twice, at most 64 and one a page."""
     from flyweight_b200.kernels import attention
     rule = attention.shared_prefix_splits
-    assert rule(2, 8, 2, 7, 1, True) == (0, 8) and rule(2, 8, 2, 128, 1, True) == (296 // 8, 1)
-    assert rule(64, 8, 4, 8, 1, True)[0] == 0 and rule(64, 8, 4, 16, 1, True)[0] == 16
-    assert rule(2048, 8, 4, 8, 1, True)[0] > 0            # several rounds of blocks
-    assert rule(2, 8, 2, 7, 1, False) == (7, 1)           # the 32-bit kernels always read the shared pages once
+    assert rule(2, 8, 2, 64, 7, 1, True) == (0, 8)
+    assert rule(2, 8, 2, 128, 128, 1, True)[0] == 296 // 8         # one row tile of eight KV heads
+    assert rule(64, 8, 4, 64, 8, 1, True)[0] == 0 and rule(64, 8, 4, 64, 16, 1, True)[0] > 1
+    assert rule(2048, 8, 4, 64, 8, 1, True)[0] > 0                 # several rounds of blocks
+    assert rule(2, 8, 2, 64, 7, 1, False) == (7, 1)                # the 32-bit kernels always read the shared pages once
     for tokens in (1, 5, 300):
         for pages in (1, 9, 1000):
-            shared, own = rule(tokens, 4, 6, pages, 50, True)
+            shared, own = rule(tokens, 4, 6, 64, pages, 50, True)
             assert 0 <= shared <= min(64, pages) and own in (1, 2, 4, 8)
 
 
