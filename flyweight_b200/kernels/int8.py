@@ -80,6 +80,11 @@ def _here(name: str, x: torch.Tensor) -> None:
         raise KernelError(f"{name} is on {x.device}, the kernels are launched on cuda:{lib._device_index()}")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    start, other = a.data_ptr(), b.data_ptr()
+    return start < other + b.numel() * b.element_size() and other < start + a.numel() * a.element_size()
+
+
 def _scratch(rows: int, columns: int, device) -> torch.Tensor:
     return torch.empty(rows * (((columns + 15) & ~15) + 4), dtype=torch.uint8, device=device)
 
@@ -154,7 +159,8 @@ def _run(x, w: Int8Matrix, out, out_dtype, addend, features: int, epilogue: int,
         _product(x, w, out, addend, features, epilogue, limit)
     else:
         address, scratch = x.data_ptr(), None
-        if M > MAX_RAW or K > MAX_RAW_COLUMNS or K & 7 or address & 15:
+        # (a result over its own input: every block reads all of a row, so the integers are made first)
+        if M > MAX_RAW or K > MAX_RAW_COLUMNS or K & 7 or address & 15 or _overlap(x, out):
             held = _scratch(M, K, w._buffer.device)
             scratch = held.data_ptr()
         lib.call("fwb_linear_int8", address, is_bf16, scratch, w._address, w._scales, out.data_ptr(),
@@ -166,7 +172,7 @@ def linear_int8(x: Union[Int8Rows, torch.Tensor], w: Int8Matrix, out_dtype: torc
                 addend: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ w.T`` [M][N] in fp32 or bf16.  ``x``: integer rows, or a bf16/fp32 matrix, which is brought to integers first.
     ``addend`` (fp32 [M][N], with an fp32 result): added behind the scales; ``out`` may be the addend itself (a residual sum in
-    place)."""
+    place) or the matrix ``x``."""
     if out_dtype is _FP32:
         epilogue = 0 if addend is None else 2
     elif out_dtype is not _BF16:

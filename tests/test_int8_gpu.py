@@ -265,6 +265,24 @@ def test_rows_off_a_border_take_two_launches():
     assert torch.equal(int8.rows_int8(off).values, int8.rows_int8(off.clone()).values)
 
 
+@pytest.mark.parametrize("M", [1, 8, 9])
+def test_a_result_over_its_own_input(M):
+    """``x`` may be the result, and the addend too: every feature is made of the rows as they were."""
+    from flyweight_b200.kernels import int8
+    matrix = int8.matrix_int8(rows_of(2048, 2048, torch.bfloat16, 1).to(DEV))
+    x = rows_of(M, 2048, torch.float32).to(DEV)
+    rows = int8.rows_int8(x)
+    for addend in (False, True):
+        want = int8.linear_int8(rows, matrix, torch.float32, addend=x if addend else None)
+        here = x.clone()
+        assert int8.linear_int8(here, matrix, torch.float32, addend=here if addend else None, out=here) is here
+        assert torch.equal(here, want)
+    held = torch.cat([x, x])                                   # overlapping by a part
+    over = held.flatten()[64:64 + M * 2048].view(M, 2048)
+    want = int8.linear_int8(rows, matrix, torch.float32)
+    assert torch.equal(int8.linear_int8(held[:M], matrix, torch.float32, out=over), want)
+
+
 def test_inputs_in_32_bits_are_brought_to_integers_first():
     from flyweight_b200.kernels import int8
     for M in (1, 6, 130):
