@@ -380,12 +380,12 @@ FWB_API int fwb_attention_prefix(const void* q, const void* k_pool, const void* 
                                  const float* sink, float softcap, cudaStream_t stream) {
     if (T <= 0 || n_groups <= 0) return FWB_OK;
     if (!q || !k_pool || !v_pool || !positions || !tok_seg || !block_table || !group_start || !group_pages || (splits && (!part_o || !part_ml)) ||
-        !out || n_segments <= 0 || max_pages <= 0 || num_pages <= 0 || splits < 0 || !(softcap >= 0.0f) ||
+        !out || n_segments <= 0 || max_pages <= 0 || num_pages <= 0 || splits < 0 || !(scale > 0.0f && scale < INFINITY) ||
+        !(softcap >= 0.0f && softcap < INFINITY) || !(softcap / scale < INFINITY) ||
         (own_slices != 1 && own_slices != 2 && own_slices != 4 && own_slices != 8))
         return FWB_BAD_ARGUMENT;
     if (nkv <= 0 || nh <= 0 || nh % nkv || hd < 1 || hd > 256) return FWB_UNSUPPORTED;
     if (nkv > 4095 || max_pages > 33554431 || splits > MAX_SPLITS) return FWB_TOO_LARGE;
-    if (softcap > 0.0f && scale == 0.0f) return FWB_UNSUPPORTED;
     Params prm{};
     prm.b = Batch{positions, tok_seg, block_table, group_start, group_pages, T, n_segments, n_groups, max_pages, num_pages};
     if (is_bf16 && tensor_cores_take(q, k_pool, v_pool, out, part_o, prm.b, nkv, hd))

@@ -317,6 +317,7 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     the keys up to its position, in shared and own pages alike, whatever the number of tokens a request has in the step; the
     result is ``paged_attention``'s.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
     position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are in ``out``.
+    ``scale`` is positive.
 
     ``sink``: fp32 [n_heads], a score per head that joins every softmax denominator (not scaled, not capped, no value);
     ``softcap`` > 0: scores become ``softcap * tanh(score / softcap)`` behind the scale.
@@ -356,15 +357,21 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
         raise KernelError(f"{groups} groups need {groups + 1} starts, got {group_start.numel()}")
     if sink is not None:
         check_tensor("sink", sink, torch.float32, (n_heads,))
-    if not softcap >= 0:
-        raise KernelError("a soft-cap must not be negative")
+    if not 0 < scale < math.inf:
+        raise KernelError(f"the scale must be a positive number, got {scale}")
+    if not 0 <= softcap < math.inf:
+        raise KernelError(f"a soft-cap must be 0 (off) or a positive number, got {softcap}")
+    if (shared_pages is not None and shared_pages < 0) or (own_pages is not None and own_pages < 0):
+        raise KernelError("shared and own pages must not be negative")
     if out is None:
         out = torch.empty_like(q)
     else:
         check_tensor("attention output", out, dtype, q.shape)
     if T == 0 or groups == 0:
         return out
-    wide = dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
+    # the tensor cores' kernels fetch rows of pools that 31 bits number, from borders of 16 bytes
+    wide = (dtype is torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128 and (num_pages + 1) * n_kv * 64 < 1 << 31
+            and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) & 15)
     splits, own = shared_prefix_splits(T, n_kv, n_heads // n_kv, head_dim, width if shared_pages is None else min(width, shared_pages),
                                        width if own_pages is None else own_pages, wide, groups)
     part_ml = part_o = None

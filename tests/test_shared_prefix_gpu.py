@@ -234,6 +234,29 @@ def test_the_rule_of_the_cut():
             assert 0 <= shared <= min(64, pages) and own in (1, 2, 4, 8)
 
 
+@pytest.mark.parametrize("which", ["q", "k_pool", "v_pool", "out"])
+def test_tensors_off_a_border(which):
+    """Storage that starts two bytes behind a border of 16 takes the kernels that read value by value."""
+    from flyweight_b200.kernels import attention
+    case = Case(BATCHES["two"], 8, 2, 64, torch.bfloat16)
+    d = case.device()
+    held = torch.full((d[which].numel() + 1,), FILL, dtype=torch.bfloat16, device=DEV)
+    held[1:] = d[which].flatten()
+    d[which] = held[1:].view(d[which].shape)
+    assert d[which].data_ptr() % 16 and d[which].is_contiguous()
+    case.check(attention.shared_prefix_attention(**d))
+    assert which != "out" or held[0] == FILL
+
+
+@pytest.mark.parametrize("more", [dict(scale=0.0), dict(scale=-0.125), dict(scale=math.nan), dict(scale=math.inf),
+                                  dict(softcap=math.inf), dict(shared_pages=-1), dict(own_pages=-1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_numbers_that_are_refused(dtype, more):
+    from flyweight_b200.kernels import KernelError
+    with pytest.raises(KernelError):
+        attend(Case(BATCHES["two"], 4, 2, 64, dtype), **more)
+
+
 def test_no_groups_and_no_tokens():
     case = Case(BATCHES["two"], 4, 4, 64, torch.bfloat16)
     d = case.device()
