@@ -357,6 +357,8 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
         raise KernelError(f"{groups} groups need {groups + 1} starts, got {group_start.numel()}")
     if sink is not None:
         check_tensor("sink", sink, torch.float32, (n_heads,))
+        if sink.get_device() != device:
+            raise KernelError(f"sink is on {sink.device}, the kernels are launched on cuda:{device}")
     if not 0 < scale < math.inf:
         raise KernelError(f"the scale must be a positive number, got {scale}")
     if not 0 <= softcap < math.inf:
@@ -367,6 +369,8 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
         out = torch.empty_like(q)
     else:
         check_tensor("attention output", out, dtype, q.shape)
+        if out.get_device() != device:
+            raise KernelError(f"attention output is on {out.device}, the kernels are launched on cuda:{device}")
     if T == 0 or groups == 0:
         return out
     # the tensor cores' kernels fetch rows of pools that 31 bits number, from borders of 16 bytes

@@ -122,12 +122,15 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
     if _input("residual", x):
         raise KernelError("the residual must be float32")
     check_tensor("norm weight", weight, _FP32, (x.shape[1],))
+    _here("norm weight", weight)
     if delta is not None:
         check_tensor("delta", delta, _FP32, x.shape)
+        _here("delta", delta)
         if rows is not None:
             raise KernelError("a residual sum goes over every row: delta and rows exclude each other")
     if rows is not None:
         check_tensor("row indices", rows, torch.int32)
+        _here("row indices", rows)
     return _quantize(x, 0, delta, weight, rows, float(eps), Int8Rows)
 
 
@@ -148,12 +151,14 @@ def _run(x, w: Int8Matrix, out, out_dtype, addend, features: int, epilogue: int,
     _here("weight", w._buffer)
     if addend is not None:
         check_tensor("product addend", addend, _FP32, (M, features))
+        _here("product addend", addend)
         if out is None:
             out = torch.empty_like(addend)
     if out is None:
         out = torch.empty((M, features), dtype=out_dtype, device=w._buffer.device)
     elif out is not addend:
         check_tensor("product output", out, out_dtype, (M, features))
+        _here("product output", out)
     if ready:
         _here("rows", x._buffer)
         _product(x, w, out, addend, features, epilogue, limit)
