@@ -34,6 +34,8 @@ struct Batch {
         const int seg = tok_seg[token];
         return seg < 0 || seg >= n_segments ? nullptr : block_table + (size_t)seg * max_pages;
     }
+    // the last key that a token at this position sees
+    __device__ __forceinline__ int last_key(int position) const { return position < max_pages * PAGE ? position : max_pages * PAGE - 1; }
     __device__ __forceinline__ bool is_page(int page) const { return page >= 0 && page < num_pages; }
 };
 
@@ -82,23 +84,28 @@ inline long most_token_tiles(int T, int n_groups, int per_tile) {
 // sees.  Asked by whole warps; the group's arrays and the token's are asked for at once.
 struct Token {
     int pages, last;
+    int first, end;              // its group's tokens
     const int* table;
 };
 __device__ __forceinline__ Token token_of(const Batch& b, int token) {
     const int lane = threadIdx.x & 31;
     const int seg = b.tok_seg[token], position = b.positions[token];
-    Token t{-1, -1, nullptr};
+    Token t{-1, -1, 0, 0, nullptr};
     for (int g0 = 0; g0 <= b.n_groups; g0 += 32) {
         const int g = g0 + lane;
-        const bool begun = g <= b.n_groups && b.start_of(g) <= token;
+        const int start = g <= b.n_groups ? b.start_of(g) : b.T;
+        const bool begun = g <= b.n_groups && start <= token;
         const int pages = g < b.n_groups ? b.pages_of(g) : -1;       // (behind the last group: in none)
         const int n = __popc(__ballot_sync(0xffffffffu, begun));
-        if (n > 0) t.pages = __shfl_sync(0xffffffffu, pages, n - 1);
-        if (n < 32) break;
+        if (n > 0) t.pages = __shfl_sync(0xffffffffu, pages, n - 1), t.first = __shfl_sync(0xffffffffu, start, n - 1);
+        if (n < 32) {
+            t.end = __shfl_sync(0xffffffffu, start, n);
+            break;
+        }
     }
     if (seg >= 0 && seg < b.n_segments) {
         t.table = b.block_table + (size_t)seg * b.max_pages;
-        t.last = position < b.max_pages * PAGE ? position : b.max_pages * PAGE - 1;
+        t.last = b.last_key(position);
     }
     return t;
 }

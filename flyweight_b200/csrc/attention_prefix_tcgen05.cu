@@ -459,6 +459,24 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 1);
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
+// The tokens that a CTA takes together: up to `most` neighbours of one request in one group, cut off from the first of them on.
+// Asked by whole warps with the request of token `t + most - 1 - lane` (anything where there is no such token).
+// 0: token t is not the first of such a piece.
+__device__ __forceinline__ int run_of(const Batch& b, const Token& token, int t, int most, int seg_around) {
+    if (!token.table) return 1;
+    const int lane = threadIdx.x & 31, seg = __shfl_sync(0xffffffffu, seg_around, most - 1);
+    const int at = t + most - 1 - lane;
+    const unsigned same = __ballot_sync(0xffffffffu, at >= token.first && at < token.end && seg_around == seg);
+    int before = __ffs(~(same >> most)) - 1, inside = t - (32 - most);
+    for (bool more = before == 32 - most; more;) {
+        inside -= 32;
+        const int back = inside + 31 - lane;
+        const int n = __ffs(~__ballot_sync(0xffffffffu, back >= token.first && b.tok_seg[back] == seg)) - 1;
+        more = n < 0;                                      // all thirty-two
+        before += more ? 32 : n;
+    }
+    return before % most ? 0 : 1 + __clz(~(same << (33 - most)));
+}
 // 2^(m - of), 0 for a part that has seen nothing
 __device__ __forceinline__ float part_weight(float m, float of) { return m == -INFINITY ? 0.0f : ex2(m - of); }
 
@@ -469,7 +487,7 @@ struct OwnLayout {
     static constexpr int data(int stages) { return stages * STAGE > MERGE_FLOATS * 4 ? stages * STAGE : MERGE_FLOATS * 4; }
 };
 
-template <int HD>
+template <int HD, bool TOGETHER>          // TOGETHER: a CTA takes neighbouring tokens of a request, as many as have rows (else one)
 __global__ void __launch_bounds__(OWN_THREADS, HD == 64 ? 4 : 3)
 own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params prm) {
     using L = OwnLayout<HD>;
@@ -496,12 +514,27 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     const int t = blockIdx.x, chunks = (prm.group + OWN_ROWS - 1) / OWN_ROWS;
     const int kvh = blockIdx.y / chunks, head0 = kvh * prm.group + (blockIdx.y % chunks) * OWN_ROWS;
     const int heads = min(OWN_ROWS, (kvh + 1) * prm.group - head0);
+    int seg_around = -1, position = -1, most = 1;
+    if constexpr (TOGETHER) {
+        most = OWN_ROWS / prm.group;
+        const int around = t + most - 1 - lane;
+        if (around >= 0 && around < prm.b.T) seg_around = prm.b.tok_seg[around];
+        if (lane < most && t + lane < prm.b.T) position = prm.b.positions[t + lane];
+    }
     const Token token = token_of(prm.b, t);
-    if (token.pages < 0) {                                 // rows of no group stay as they are; the whole cluster leaves
+    const int tokens = TOGETHER ? run_of(prm.b, token, t, most, seg_around) : 1;
+    if (token.pages < 0 || tokens == 0) {                  // rows of no group stay as they are; the whole cluster leaves
         pdl_wait();
         return;
     }
-    const int pages = prm.alone ? 0 : token.pages, last = token.last;
+    // rows: token, head.  `sees`: the last key that this lane's token sees
+    const int rows = tokens * heads, pages = prm.alone ? 0 : token.pages;
+    int sees = token.last, last = token.last, least = token.last;
+    if constexpr (TOGETHER) {
+        sees = token.table ? prm.b.last_key(position) : -1;
+        last = __reduce_max_sync(0xffffffffu, lane < tokens ? sees : -1);
+        least = __reduce_min_sync(0xffffffffu, lane < tokens ? sees : 0x7fffffff);
+    }
     const int* table = token.table;
     const int own = last >= pages * KEYS ? last / KEYS + 1 - pages : 0, per = (own + slices - 1) / slices;
     const int tile0 = pages + slice * per, tile1 = min(pages + own, tile0 + per), n_tiles = max(0, tile1 - tile0);
@@ -537,13 +570,18 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         }
     } else if (n_tiles > 0) {
         uint32_t qf[HD / 16][4];
+        int token_of_row[2] = {0, 0}, sees_of_row[2] = {last, last};
+        if constexpr (TOGETHER) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) token_of_row[i] = (g + 8 * i) / heads, sees_of_row[i] = __shfl_sync(0xffffffffu, sees, token_of_row[i]);
+        }
         const __nv_bfloat16* q_at = prm.q + ((size_t)t * prm.nh + head0) * prm.hd;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = g + (i & 1) * 8, c = kk * 16 + (i >> 1) * 8 + t4 * 2;
-                qf[kk][i] = r < heads && c < prm.hd ? *reinterpret_cast<const uint32_t*>(q_at + (size_t)r * prm.hd + c) : 0u;
+                const int r = g + (i & 1) * 8, c = kk * 16 + (i >> 1) * 8 + t4 * 2, j = token_of_row[i & 1];
+                qf[kk][i] = r < rows && c < prm.hd ? *reinterpret_cast<const uint32_t*>(q_at + ((size_t)j * prm.nh + r - j * heads) * prm.hd + c) : 0u;
             }
         const int key_k = warp * 16 + (lane >> 4) * 8 + (lane & 7), chunk_k = (lane >> 3) & 1;     // ldmatrix rows of K and V
         const int key_v = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), chunk_v = lane >> 4;
@@ -570,12 +608,12 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sc[n][i] = prm.cap_unit * tanh_fast_f32(sc[n][i] * prm.cap_pre);
                 }
-                const bool whole = key0 + 15 <= last;
+                const bool whole = key0 + 15 <= least, mixed = TOGETHER && least < min(last, key0 + 15);
                 if (!whole) {
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[n][i] = key0 + n * 8 + t4 * 2 + (i & 1) <= last ? sc[n][i] : -INFINITY;
+                        for (int i = 0; i < 4; ++i) sc[n][i] = key0 + n * 8 + t4 * 2 + (i & 1) <= sees_of_row[i >> 1] ? sc[n][i] : -INFINITY;
                     // the values of keys that nobody sees, whatever they hold (the slice's last tile: nothing is copied over it)
                     for (int i = lane; i < (15 - (last - key0)) * 8 * L::BOXES; i += 32) {
                         const int r = warp * 16 + (last - key0) + 1 + (i >> 3) % (15 - (last - key0));
@@ -606,13 +644,38 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i) o[i][0] *= factor[0], o[i][1] *= factor[0], o[i][2] *= factor[1], o[i][3] *= factor[1];
                 }
-#pragma unroll
-                for (int n = 0; n < HD / 8; n += 2) {
-                    uint32_t b[4];
+                auto values = [&](uint32_t (&b)[4], int n) {
                     const int chunk = (n + chunk_v) & 7;
                     ldmatrix_x4_trans(b, v_at + (n >> 3) * KV_BOX + key_v * 128 + ((chunk ^ (key_v & 7)) << 4));
-                    mma_bf16(o[n], p0, p1, p2, p3, b[0], b[1]);
-                    mma_bf16(o[n + 1], p0, p1, p2, p3, b[2], b[3]);
+                };
+                if (!mixed) {
+#pragma unroll
+                    for (int n = 0; n < HD / 8; n += 2) {
+                        uint32_t b[4];
+                        values(b, n);
+                        mma_bf16(o[n], p0, p1, p2, p3, b[0], b[1]);
+                        mma_bf16(o[n + 1], p0, p1, p2, p3, b[2], b[3]);
+                    }
+                } else {
+                    // some of the tokens see all of these keys: a token at a time, with the values that it sees and for its rows
+#pragma unroll 1
+                    for (int j = 0; j < tokens; ++j) {
+                        const int seen = __shfl_sync(0xffffffffu, sees, j) - key0 - 2 * t4;
+                        const uint32_t front = (seen >= 0 ? 0xffffu : 0u) | (seen >= 1 ? 0xffff0000u : 0u);
+                        const uint32_t behind = (seen >= 8 ? 0xffffu : 0u) | (seen >= 9 ? 0xffff0000u : 0u);
+#pragma unroll
+                        for (int n = 0; n < HD / 8; n += 2) {
+                            uint32_t b[4];
+                            values(b, n);
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                float d[4] = {};
+                                mma_bf16(d, p0, p1, p2, p3, b[2 * k] & front, b[2 * k + 1] & behind);
+                                if (token_of_row[0] == j) o[n + k][0] += d[0], o[n + k][1] += d[1];
+                                if (token_of_row[1] == j) o[n + k][2] += d[2], o[n + k][3] += d[3];
+                            }
+                        }
+                    }
                 }
             }
             __syncwarp();
@@ -637,7 +700,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
             l[r] = quad_sum(l[r]);
             const int row = warp * OWN_ROWS + g + 8 * r;
             if (t4 == 0) ml_s[2 * row] = m[r], ml_s[2 * row + 1] = l[r];
-            if (g + 8 * r < heads) {
+            if (g + 8 * r < rows) {
 #pragma unroll
                 for (int n = 0; n < HD / 8; ++n)
                     *reinterpret_cast<float2*>(o_s + row * HD + n * 8 + t4 * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
@@ -658,7 +721,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         joined[row][0] = top, joined[row][1] = sum;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * HD; i += OWN_THREADS) {
+    for (int i = threadIdx.x; i < rows * HD; i += OWN_THREADS) {
         const int row = i / HD;
         float v = 0.0f;
 #pragma unroll
@@ -676,9 +739,10 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     // of them asked for at once), then the sums, eight parts' channels on the way together
     const int shared_per = pages ? pages_per_slice(pages, prm.splits) : 0, shared = pages ? (pages + shared_per - 1) / shared_per : 0;
     const uint32_t o_at = smem_u32(o_s), ml_at = smem_u32(joined);
-    for (int row = warp; row < heads; row += OWN_WARPS + 1) {
-        const size_t at = ((size_t)t * prm.nh + head0 + row) * prm.splits;
-        const float sink = prm.sink ? prm.sink[head0 + row] * LOG2E : -INFINITY;
+    for (int row = warp; row < rows; row += OWN_WARPS + 1) {
+        const int j = TOGETHER ? row / heads : 0, head = head0 + row - j * heads;
+        const size_t at = ((size_t)(t + j) * prm.nh + head) * prm.splits;
+        const float sink = prm.sink ? prm.sink[head] * LOG2E : -INFINITY;
         float2 part[(MAX_SPLITS + 31) / 32], mine = make_float2(-INFINITY, 0.0f);
         if (lane < slices) {
             mine.x = cluster ? ld_dsmem_f32(ml_at + row * 8, lane) : joined[row][0];
@@ -705,10 +769,11 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
     }
     __syncthreads();
     constexpr int LANES = HD / 4;                          // threads a row, four channels each
-    for (int i = threadIdx.x; i < heads * LANES; i += OWN_THREADS) {
-        const int row = i / LANES, c = (i - row * LANES) * 4;
+    for (int i = threadIdx.x; i < rows * LANES; i += OWN_THREADS) {
+        const int row = i / LANES, c = (i - row * LANES) * 4, j = TOGETHER ? row / heads : 0;
         if ((cluster && row % slices != slice) || c >= prm.hd) continue;
-        const float* parts = prm.part_o + ((size_t)t * prm.nh + head0 + row) * prm.splits * prm.hd + c;
+        const size_t out_row = (size_t)(t + j) * prm.nh + head0 + row - j * heads;
+        const float* parts = prm.part_o + out_row * prm.splits * prm.hd + c;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto add = [&](float f, const float4& x) {
             v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
@@ -732,7 +797,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         }
         if (!*abort_flag) {
             const float inv = inverse[row];
-            *reinterpret_cast<uint2*>(prm.out + ((size_t)t * prm.nh + head0 + row) * prm.hd + c) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+            *reinterpret_cast<uint2*>(prm.out + out_row * prm.hd + c) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
         }
     }
     if (cluster) cluster_sync_all();                       // nobody leaves while a peer still reads from it
@@ -743,12 +808,13 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int o
     using L = Layout<HD>;
     auto plain = prefix_tcgen05_kernel<HD, false>;
     auto capped = prefix_tcgen05_kernel<HD, true>;
-    auto own = own_kernel<HD>;
+    auto own = own_kernel<HD, false>, together = own_kernel<HD, true>;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(plain, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(capped, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(together, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
@@ -777,7 +843,9 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int o
     }
     config.attrs = attr;
     config.numAttrs = n;
-    cudaError_t status = cudaLaunchKernelEx(&config, own, map_k, map_v, prm);
+    // tokens of one request together where there must be some and two tokens' heads fit the rows
+    const bool runs = prm.b.T > prm.b.n_segments && 2 * prm.group <= OWN_ROWS;
+    cudaError_t status = cudaLaunchKernelEx(&config, runs ? together : own, map_k, map_v, prm);
     return status == cudaSuccess ? fwb_launch_status() : (int)status;
 }
 

@@ -152,6 +152,55 @@ def test_positions_inside_the_shared_pages_and_before_the_first(cut, dtype, dim)
     case.check(attend(case))
 
 
+RUNS = {
+    "drafts": [(2, [(3, 40), (1, 9), (4, 66), (2, 2), (5, 200)]), (1, [(7, 64), (3, 63)])],
+    "a prompt beside": [(1, [(1, 5), (77, 140), (1, 30), (33, 33)]), (0, [(100, 100), (2, 65)])],
+    "all of one": [(3, [(50, 300)])],
+}
+
+
+@pytest.mark.parametrize("batch", sorted(RUNS))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 4, 128), (3, 1, 64), (12, 3, 128), (10, 2, 80), (6, 1, 128), (7, 1, 48), (16, 2, 64),
+                                          (9, 1, 64), (16, 1, 128), (34, 2, 64)])
+def test_several_tokens_of_a_request(cut, batch, dtype, heads, kv, dim):
+    """Neighbouring tokens of a request are taken together, whatever their number and the heads of each."""
+    case = Case(RUNS[batch], heads, kv, dim, dtype, idle=2)
+    case.check(attend(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tokens_of_a_request_in_any_order(cut, dtype, dim):
+    """Positions that fall, jump, repeat or are none; a request whose tokens do not lie together; one request on both sides of a
+    border of groups."""
+    case = Case([(2, [(9, 300)]), (1, [(4, 100), (3, 20)])], 6, 2, dim, dtype)
+    case.positions[:9] = [427, 130, 131, -1, 300, 300, 129, 5, 426]
+    case.check(attend(case))
+    case = Case([(1, [(2, 50), (2, 60), (2, 70)])], 4, 2, dim, dtype)
+    case.segment = [0, 1, 0, 2, 2, 1]
+    case.positions = [64 + 48, 64 + 58, 64 + 49, 64 + 69, 64 + 68, 64 + 59]
+    case.check(attend(case))
+    case = Case([(1, [(6, 200)])], 4, 2, dim, dtype)
+    case.starts, case.pages = [0, 2, 6], [1, 0]
+    case.check(attend(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 80])
+def test_a_later_token_of_a_request_is_not_seen(cut, dtype, dim):
+    """Infinities in the value and NaN in the key of a request's last token: the tokens in front of it do not see them."""
+    case = Case([(1, [(3, 40), (1, 7), (5, 66)])], 6, 2, dim, dtype)
+    want = attend(case).clone()
+    for row, n in zip((0, 2), (64 + 40, 64 + 66)):
+        page = case.rows[row][(n - 1) // PAGE]
+        case.k[page, :, (n - 1) % PAGE], case.v[page, :, (n - 1) % PAGE] = math.nan, math.inf
+    got = attend(case)
+    seen = [0, 1, 3, 4, 5, 6, 7]
+    assert torch.equal(got[seen], want[seen])
+    assert torch.isnan(got[[2, 8]].float()).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128, 80])
 def test_what_lies_behind_the_last_key_is_not_seen(cut, dtype, dim):
