@@ -708,45 +708,48 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         }
     }
     __syncthreads();
-    // this CTA's warps together (rows stay in o_s's first quarter): every thread has channels of rows
-    if (threadIdx.x < OWN_ROWS) {
-        const int row = threadIdx.x;
-        float top = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < OWN_WARPS; ++w) top = fmaxf(top, ml_s[2 * (w * OWN_ROWS + row)]);
-        for (int w = 0; w < OWN_WARPS; ++w) {
-            const float f = part_weight(ml_s[2 * (w * OWN_ROWS + row)], top);
-            sum += f * ml_s[2 * (w * OWN_ROWS + row) + 1];
-            ml_s[2 * (w * OWN_ROWS + row)] = f;            // from here on: the warp's weight
+    const bool cluster = slices > 1;
+    if (cluster) {
+        // this CTA's warps together, for its peers to read (rows stay in o_s's first quarter): every thread has channels of rows
+        if (threadIdx.x < OWN_ROWS) {
+            const int row = threadIdx.x;
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = 0; w < OWN_WARPS; ++w) top = fmaxf(top, ml_s[2 * (w * OWN_ROWS + row)]);
+            for (int w = 0; w < OWN_WARPS; ++w) {
+                const float f = part_weight(ml_s[2 * (w * OWN_ROWS + row)], top);
+                sum += f * ml_s[2 * (w * OWN_ROWS + row) + 1];
+                ml_s[2 * (w * OWN_ROWS + row)] = f;        // from here on: the warp's weight
+            }
+            joined[row][0] = top, joined[row][1] = sum;
         }
-        joined[row][0] = top, joined[row][1] = sum;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * HD; i += OWN_THREADS) {
-        const int row = i / HD;
-        float v = 0.0f;
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * HD; i += OWN_THREADS) {
+            const int row = i / HD;
+            float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < OWN_WARPS; ++w) {
-            const float f = ml_s[2 * (w * OWN_ROWS + row)];
-            if (f != 0.0f) v = fmaf(f, o_s[(w * OWN_ROWS) * HD + i], v);
+            for (int w = 0; w < OWN_WARPS; ++w) {
+                const float f = ml_s[2 * (w * OWN_ROWS + row)];
+                if (f != 0.0f) v = fmaf(f, o_s[(w * OWN_ROWS) * HD + i], v);
+            }
+            o_s[i] = v;
         }
-        o_s[i] = v;
     }
     pdl_wait();                  // the shared part is there
-    const bool cluster = slices > 1;
     if (cluster) cluster_sync_all();
-    else __syncthreads();
-    // the join: with a cluster every CTA has a share of the rows.  First the parts' weights, a warp a row and a lane a part (all
-    // of them asked for at once), then the sums, eight parts' channels on the way together
+    // the join: of the warps' parts, or with a cluster of the CTAs', each of which has a share of the rows.  First the parts'
+    // weights, a warp a row and a lane a part (all of them asked for at once), then the sums, eight parts' channels on the way
+    // together
     const int shared_per = pages ? pages_per_slice(pages, prm.splits) : 0, shared = pages ? (pages + shared_per - 1) / shared_per : 0;
+    const int own_parts = cluster ? slices : OWN_WARPS;
     const uint32_t o_at = smem_u32(o_s), ml_at = smem_u32(joined);
     for (int row = warp; row < rows; row += OWN_WARPS + 1) {
         const int j = TOGETHER ? row / heads : 0, head = head0 + row - j * heads;
         const size_t at = ((size_t)(t + j) * prm.nh + head) * prm.splits;
         const float sink = prm.sink ? prm.sink[head] * LOG2E : -INFINITY;
         float2 part[(MAX_SPLITS + 31) / 32], mine = make_float2(-INFINITY, 0.0f);
-        if (lane < slices) {
-            mine.x = cluster ? ld_dsmem_f32(ml_at + row * 8, lane) : joined[row][0];
-            mine.y = cluster ? ld_dsmem_f32(ml_at + row * 8 + 4, lane) : joined[row][1];
+        if (lane < own_parts) {
+            mine.x = cluster ? ld_dsmem_f32(ml_at + row * 8, lane) : ml_s[2 * (lane * OWN_ROWS + row)];
+            mine.y = cluster ? ld_dsmem_f32(ml_at + row * 8 + 4, lane) : ml_s[2 * (lane * OWN_ROWS + row) + 1];
         }
         float top = fmaxf(sink, mine.x);
 #pragma unroll
@@ -757,7 +760,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
         top = warp_max(top);
         const float f = part_weight(mine.x, top);
         float sum = f * mine.y + (lane == 0 ? part_weight(sink, top) : 0.0f);
-        if (lane < slices) own_weight[row][lane] = f;
+        if (lane < own_parts) own_weight[row][lane] = f;
 #pragma unroll
         for (int i = 0; i < (MAX_SPLITS + 31) / 32; ++i) {
             const float w = part_weight(part[i].x, top);
@@ -790,10 +793,10 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
 #pragma unroll
             for (int k = 0; k < 8; ++k) add(f[k], x[k]);
         }
-        for (int s = 0; s < slices; ++s) {
+        for (int s = 0; s < own_parts; ++s) {
             const float f = own_weight[row][s];
             if (f == 0.0f) continue;
-            add(f, cluster ? ld_dsmem_f32x4(o_at + (uint32_t)(row * HD + c) * 4, s) : *reinterpret_cast<const float4*>(o_s + row * HD + c));
+            add(f, cluster ? ld_dsmem_f32x4(o_at + (uint32_t)(row * HD + c) * 4, s) : *reinterpret_cast<const float4*>(o_s + (s * OWN_ROWS + row) * HD + c));
         }
         if (!*abort_flag) {
             const float inv = inverse[row];
