@@ -371,12 +371,13 @@ int launch(const Params& prm, cudaStream_t stream) {
 // q, out: [T][nh * hd]; pools [num_pages][nkv][64][hd]; all bf16 or all fp32.  positions, tok_seg: [T]; block_table:
 // [n_segments][max_pages]; group_start: [n_groups + 1], group_pages: [n_groups]; part_o: fp32 [T][nh][splits][hd], part_ml: fp32
 // [T][nh][splits][2], scratch.  sink: [nh] or null; softcap 0: off.  own_slices (1, 2, 4, 8): how many CTAs share a token's own keys
-// on the tensor cores.  splits 0 (on the tensor cores): without the prefix kernel and its scratch, every
+// on the tensor cores.  neighbours: there, neighbouring tokens of a request are taken together where two have at most sixteen query
+// heads of a KV head.  splits 0 (on the tensor cores): without the prefix kernel and its scratch, every
 // token walks the shared pages by itself.
 FWB_API int fwb_attention_prefix(const void* q, const void* k_pool, const void* v_pool, int is_bf16, const int* positions,
                                  const int* tok_seg, const int* block_table, int n_segments, int max_pages, int num_pages,
                                  const int* group_start, const int* group_pages, int n_groups, float* part_o, float* part_ml,
-                                 void* out, int T, int nh, int nkv, int hd, int splits, int own_slices, float scale,
+                                 void* out, int T, int nh, int nkv, int hd, int splits, int own_slices, int neighbours, float scale,
                                  const float* sink, float softcap, cudaStream_t stream) {
     if (T <= 0 || n_groups <= 0) return FWB_OK;
     if (!q || !k_pool || !v_pool || !positions || !tok_seg || !block_table || !group_start || !group_pages || (splits && (!part_o || !part_ml)) ||
@@ -389,7 +390,8 @@ FWB_API int fwb_attention_prefix(const void* q, const void* k_pool, const void* 
     Params prm{};
     prm.b = Batch{positions, tok_seg, block_table, group_start, group_pages, T, n_segments, n_groups, max_pages, num_pages};
     if (is_bf16 && tensor_cores_take(q, k_pool, v_pool, out, part_o, prm.b, nkv, hd))
-        return launch_tensor_cores(prm.b, q, k_pool, v_pool, out, part_o, part_ml, sink, nh, nkv, hd, splits, own_slices, scale, softcap, stream);
+        return launch_tensor_cores(prm.b, q, k_pool, v_pool, out, part_o, part_ml, sink, nh, nkv, hd, splits, own_slices,
+                                   neighbours && 2 * (nh / nkv) <= 16, scale, softcap, stream);
     if (splits == 0) return FWB_UNSUPPORTED;
     prm.q = q, prm.k = k_pool, prm.v = v_pool, prm.part_o = part_o, prm.part_ml = part_ml, prm.out = out, prm.sink = sink;
     prm.nh = nh, prm.nkv = nkv, prm.group = nh / nkv, prm.hd = hd, prm.splits = splits;

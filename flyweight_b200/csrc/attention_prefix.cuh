@@ -116,7 +116,7 @@ __host__ __device__ __forceinline__ int pages_per_slice(int pages, int splits) {
 // The bfloat16 form on tensor cores (host functions, attention_prefix_tcgen05.cu): whether it takes the shape, and its launch.
 bool tensor_cores_take(const void* q, const void* k_pool, const void* v_pool, const void* out, const void* part_o, const Batch& b, int nkv, int hd);
 int launch_tensor_cores(const Batch& b, const void* q, const void* k_pool, const void* v_pool, void* out, float* part_o, float* part_ml,
-                        const float* sink, int nh, int nkv, int hd, int splits, int own_slices, float scale, float softcap,
+                        const float* sink, int nh, int nkv, int hd, int splits, int own_slices, bool neighbours, float scale, float softcap,
                         cudaStream_t stream);
 
 }  // namespace prefix

@@ -807,7 +807,7 @@ own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CU
 }
 
 template <int HD>
-int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int own_slices, cudaStream_t stream) {
+int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int own_slices, bool neighbours, cudaStream_t stream) {
     using L = Layout<HD>;
     auto plain = prefix_tcgen05_kernel<HD, false>;
     auto capped = prefix_tcgen05_kernel<HD, true>;
@@ -846,9 +846,7 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, Params prm, int o
     }
     config.attrs = attr;
     config.numAttrs = n;
-    // tokens of one request together where there must be some and two tokens' heads fit the rows
-    const bool runs = prm.b.T > prm.b.n_segments && 2 * prm.group <= OWN_ROWS;
-    cudaError_t status = cudaLaunchKernelEx(&config, runs ? together : own, map_k, map_v, prm);
+    cudaError_t status = cudaLaunchKernelEx(&config, neighbours ? together : own, map_k, map_v, prm);
     return status == cudaSuccess ? fwb_launch_status() : (int)status;
 }
 
@@ -863,7 +861,7 @@ bool tensor_cores_take(const void* q, const void* k_pool, const void* v_pool, co
 }
 
 int launch_tensor_cores(const Batch& b, const void* q, const void* k_pool, const void* v_pool, void* out, float* part_o, float* part_ml,
-                        const float* sink, int nh, int nkv, int hd, int splits, int own_slices, float scale, float softcap,
+                        const float* sink, int nh, int nkv, int hd, int splits, int own_slices, bool neighbours, float scale, float softcap,
                         cudaStream_t stream) {
     Params prm{};
     prm.b = b;
@@ -881,7 +879,8 @@ int launch_tensor_cores(const Batch& b, const void* q, const void* k_pool, const
     prm.status = status_word();
     CUtensorMap map_k, map_v;
     if (!make_map(&map_k, k_pool, rows, hd, KEYS) || !make_map(&map_v, v_pool, rows, hd, KEYS)) return FWB_UNSUPPORTED;
-    return hd <= 64 ? launch<64>(map_k, map_v, prm, own_slices, stream) : launch<128>(map_k, map_v, prm, own_slices, stream);
+    return hd <= 64 ? launch<64>(map_k, map_v, prm, own_slices, neighbours, stream)
+                    : launch<128>(map_k, map_v, prm, own_slices, neighbours, stream);
 }
 
 }  // namespace prefix

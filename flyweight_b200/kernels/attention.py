@@ -305,6 +305,15 @@ def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, head_dim: int, sh
     return shared, own
 
 
+def neighbours_together(n_tokens: int, requests: int, n_kv: int) -> bool:
+    """Whether ``shared_prefix_attention`` reads a request's own keys once for its neighbouring tokens instead of once a token: with
+    more tokens than requests, and more blocks than fit the SMs at once."""
+    # Measured on B200 (us, behind 32 shared pages, up to 700 own keys, once a token and together): 32 heads over 8 of 64, 4 tokens of
+    # 16 32 64 requests 25.5 28.6, 37.7 35.3, 62.5 51.7; 8 over 4 of 128, 32 64 requests 34.7 37.0, 51.8 45.0.  The join of several
+    # tokens' rows takes 2 to 4 us more.
+    return n_tokens > requests and n_tokens * n_kv > 6 * SM_COUNT
+
+
 def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, group_start, group_pages, n_heads: int,
                             scale: float, sink=None, softcap: float = 0.0, out=None, shared_pages=None, own_pages=None):
     """Causal GQA of a batch whose requests share their first pages -- a system prompt, one prompt's many answers -- with
@@ -389,5 +398,5 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     lib.call("fwb_attention_prefix", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), 1 if dtype is torch.bfloat16 else 0,
              positions.data_ptr(), tok_seg.data_ptr(), block_table.data_ptr(), requests, width, num_pages, group_start.data_ptr(),
              group_pages.data_ptr(), groups, part_o, part_ml, out.data_ptr(), T, n_heads, n_kv, head_dim,
-             splits, own, scale, lib.ptr(sink), softcap, lib.stream(), launches=2 if splits else 1)
+             splits, own, 1 if neighbours_together(T, requests, n_kv) else 0, scale, lib.ptr(sink), softcap, lib.stream(), launches=2 if splits else 1)
     return out

@@ -159,11 +159,26 @@ RUNS = {
 }
 
 
+@pytest.fixture(params=["together", "one by one"])
+def neighbours(request, monkeypatch):
+    """The rule takes neighbours together in large batches only."""
+    from flyweight_b200.kernels import attention
+    monkeypatch.setattr(attention, "neighbours_together", lambda *sizes: request.param == "together")
+
+
+def test_neighbours_are_taken_together_in_large_batches():
+    from flyweight_b200.kernels.attention import neighbours_together
+    assert neighbours_together(256, 64, 8) and neighbours_together(295, 96, 4)
+    assert not neighbours_together(64, 16, 8) and not neighbours_together(256, 256, 8)
+    case = Case([(2, [(4, 30 + i) for i in range(64)])], 8, 4, 64, torch.bfloat16)
+    case.check(attend(case))
+
+
 @pytest.mark.parametrize("batch", sorted(RUNS))
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 4, 128), (3, 1, 64), (12, 3, 128), (10, 2, 80), (6, 1, 128), (7, 1, 48), (16, 2, 64),
                                           (9, 1, 64), (16, 1, 128), (34, 2, 64)])
-def test_several_tokens_of_a_request(cut, batch, dtype, heads, kv, dim):
+def test_several_tokens_of_a_request(cut, neighbours, batch, dtype, heads, kv, dim):
     """Neighbouring tokens of a request are taken together, whatever their number and the heads of each."""
     case = Case(RUNS[batch], heads, kv, dim, dtype, idle=2)
     case.check(attend(case))
@@ -171,7 +186,7 @@ def test_several_tokens_of_a_request(cut, batch, dtype, heads, kv, dim):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_tokens_of_a_request_in_any_order(cut, dtype, dim):
+def test_tokens_of_a_request_in_any_order(cut, neighbours, dtype, dim):
     """Positions that fall, jump, repeat or are none; a request whose tokens do not lie together; one request on both sides of a
     border of groups."""
     case = Case([(2, [(9, 300)]), (1, [(4, 100), (3, 20)])], 6, 2, dim, dtype)
@@ -188,7 +203,7 @@ def test_tokens_of_a_request_in_any_order(cut, dtype, dim):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128, 80])
-def test_a_later_token_of_a_request_is_not_seen(cut, dtype, dim):
+def test_a_later_token_of_a_request_is_not_seen(cut, neighbours, dtype, dim):
     """Infinities in the value and NaN in the key of a request's last token: the tokens in front of it do not see them."""
     case = Case([(1, [(3, 40), (1, 7), (5, 66)])], 6, 2, dim, dtype)
     want = attend(case).clone()
