@@ -286,19 +286,31 @@ def shared_prefix_splits(n_tokens: int, n_kv: int, group: int, head_dim: int, sh
             own *= 2
         if -(-shared_pages // own) * -(-pairs // (4 * SM_COUNT)) <= 8:
             return 0, own
-    # A slice's walk takes 0.63 us a page (1.1 at head sizes above 64, 2 in fp32), and its results 1 us a megabyte, there and back:
-    # 64 requests, 8 heads over 2 of 128, 128 pages in 8 16 32 64 slices 30.7 22.4 20.2 27.0; 2 requests, 16 heads over 8 of 64, 512 pages
-    # in 8 16 32 64 slices 52.1 32.0 27.2 33.2.  Not more blocks than the SMs hold at once; the tiles of a group are its own, half a
-    # tile more for every further group (53 requests of three tokens in six groups, counted without: two rounds, 62.8; with, 58.3).
+    # A slice's walk takes 0.45 us a page (1.0 at head sizes above 64, 2 in fp32), its results 0.4 us a megabyte (1), there and back, and
+    # 0.04 more to be joined.  Not more blocks than the SMs hold at once; the tiles of a group are its own, half a tile more for every
+    # further group.  Two blocks on an SM take its place from the own kernel, which otherwise starts beside them: 2 us, where that
+    # kernel's blocks would all find one.  Measured on B200 (us, requests of one token): 64, 32 heads over 8 of 64, 128 pages in 8 11 16 18
+    # 24 slices 28.2 28.2 26.9 27.3 35.3; 4 of the same, 10 13 16 18 21 32 slices 18.9 15.8 14.7 15.3 19.3 17.5, with 400 pages 16 18 24 34
+    # 43 slices 29.1 28.7 29.0 26.3 31.7; 128 requests, 24 heads over 4 of 128, 128 pages in 4 6 8 10 16 slices 65.2 57.5 51.2 52.0 63.4.
+    # Over 58 such sweeps the rule's cut takes 2 % more than the best one on average, 16 % at most.
     rows = 128 if wide else 64
     chunk = min(group, rows)
     row_tiles = (-(-n_tokens // (rows // chunk)) + (groups - 1) // 2) * -(-group // chunk) * n_kv
-    page_us = 2.0 if not wide else 0.63 if head_dim <= 64 else 1.1
-    best = math.sqrt(page_us * shared_pages / (4e-6 * n_tokens * n_kv * group * head_dim))
-    shared = max(1, min(shared_pages, 64, 2 * SM_COUNT // row_tiles, round(best)))
-    if wide and head_dim <= 64:
-        per = -(-shared_pages // shared)
-        shared = -(-shared_pages // (per + (per & 1)))         # steps of two pages
+    page_us = 2.0 if not wide else 0.45 if head_dim <= 64 else 1.0
+    slice_us = (0.4 if wide else 1.0) * 4e-6 * n_tokens * n_kv * group * head_dim + 0.04
+    step = 2 if wide and head_dim <= 64 else 1                 # pages a step
+
+    def cut(slices):
+        per = max(1, -(-shared_pages // max(1, min(shared_pages, 64, slices))))
+        per += per % step
+        return -(-shared_pages // per), per
+
+    shared, per = cut(min(2 * SM_COUNT // row_tiles, round(math.sqrt(page_us * shared_pages / slice_us))))
+    if wide and shared * row_tiles > SM_COUNT and pairs <= SM_COUNT:
+        fewer, longer = cut(SM_COUNT // row_tiles)
+        if longer * page_us + fewer * slice_us < per * page_us + shared * slice_us + 2.0:
+            shared = fewer
+    shared = max(1, shared)
     own = 1
     while own < 8 and pairs * own * 2 <= 2 * SM_COUNT and own_pages >= 8 * own:
         own *= 2
@@ -324,7 +336,7 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     ``group_start[g + 1]`` (int32 [groups + 1], rising) are group g's; the block-table rows of its requests begin with the same
     ``group_pages[g]`` pages (int32 [groups]; 0: nothing shared), named by the row of its first token.  Every token sees
     the keys up to its position, in shared and own pages alike, whatever the number of tokens a request has in the step; the
-    result is ``paged_attention``'s.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
+    result is ``paged_attention``'s.  Shared values that one of a group's tokens sees must be finite.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
     position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are in ``out``.
     ``scale`` is positive.
 

@@ -284,11 +284,12 @@ def test_pages_outside_the_pool_are_not_read(cut, dtype):
 
 def test_the_rule_of_the_cut():
     """Few shared pages a block: one launch; else slices by what walking a page and what a slice's results cost, not more than fill
-    the SMs twice, at most 64 and one a page."""
+    the SMs twice (once, where that leaves room for the kernel behind), at most 64 and one a page."""
     from flyweight_b200.kernels import attention
     rule = attention.shared_prefix_splits
     assert rule(2, 8, 2, 64, 7, 1, True) == (0, 8)
-    assert rule(2, 8, 2, 128, 128, 1, True)[0] == 296 // 8         # one row tile of eight KV heads
+    assert rule(2, 8, 2, 128, 128, 1, True)[0] == 32               # one row tile of eight KV heads: 37 slices at most, 4 pages each
+    assert rule(4, 8, 4, 64, 128, 4, True)[0] == 16                # 128 blocks, beside which the own kernel's find room
     assert rule(64, 8, 4, 64, 8, 1, True)[0] == 0 and rule(64, 8, 4, 64, 16, 1, True)[0] > 1
     assert rule(2048, 8, 4, 64, 8, 1, True)[0] > 0                 # several rounds of blocks
     assert rule(2, 8, 2, 64, 7, 1, False) == (7, 1)                # the 32-bit kernels always read the shared pages once
