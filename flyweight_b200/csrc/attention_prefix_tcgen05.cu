@@ -6,14 +6,22 @@
 //                   read from tensor memory.  The scores of a step are computed while the softmax works on those of the
 //                   step before, which it holds in registers.  m follows the running maximum only when that has grown by
 //                   more than 2^8.  Leaves m (in base 2), l and O, not divided, of its slice in scratch, fp32.
-//   own kernel      a CTA: one token, up to 16 query heads of one KV head (the rows of mma.sync 16 x 8 x 16), one slice of the keys behind
-//                   the shared ones; four warps take 16 keys each of every 64-key tile that TMA brings, with a running
-//                   maximum and sum each.  The warps' results meet in shared memory, the slices' in a cluster, the shared
-//                   part's slices from scratch (or, alone, all keys are its own): m = max m_i, O = sum 2^(m_i - m) O_i, l likewise; a sink joins m and l.
+//   own kernel      a CTA: one token and up to 16 query heads of one KV head (the rows of mma.sync 16 x 8 x 16), in large batches
+//                   as many neighbouring tokens of a request as have room there, one slice of the keys behind the shared ones;
+//                   four warps take 16 keys each of every 64-key tile that TMA brings, with a running maximum and sum each.
+//                   The warps' results meet in shared memory, the slices' in a cluster, the shared part's slices from scratch
+//                   (or, alone, all keys are its own): m = max m_i, O = sum 2^(m_i - m) O_i, l likewise; a sink joins m and l.
 //
 // The shared keys are thus read once for 128 rows.  The own kernel starts as the prefix kernel's CTAs leave and waits for them
 // only ahead of the join: the prefix kernel lets it start when it has itself waited for the kernel in front, so everything that the own
 // kernel reads before the join was written earlier than that.
+//
+// Measured on B200, bf16 (us; what the bytes take at a copy's 6.57 TB/s, the products at 1,670 TFLOP/s): 64 requests of 32 heads over 8
+// of 64 behind 8,192 keys, each with up to 500 of its own, 32.8 (7.8; 2.7): the prefix kernel 21.5, then 8 to 9 until the
+// last own keys are walked and all is joined -- blocks' latencies from arrays to pages to products, 1.5 us a page under load;
+// 256 requests behind 32,768 keys, up to 1,000 own, 178 (50.5; 41.8): 120 and 58.  The prefix kernel there is bound by what the
+// softmax issues -- the special-function pipe is 56 % busy, the tensor pipe 39 %, DRAM 5 % -- with two warps a scheduler; the own kernel reads 290 MB at 5 TB/s, four CTAs an SM.  Two prefix CTAs an SM (82 or
+// 96 KiB each, 168 registers a thread) hide one's softmax behind the other's products; three with the scores under P: slower.
 //
 // Masked keys are left out by selection; rows of V behind the last key anybody sees are cleared in shared memory, so that
 // 0 * (infinity or NaN) cannot reach a result.  A page id outside the pool is fetched as zeros and masked.
@@ -459,23 +467,23 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 1);
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-// The tokens that a CTA takes together: up to `most` neighbours of one request in one group, cut off from the first of them on.
+// The tokens that a CTA takes together: at most `most` (2 to 16) neighbours of one request in one group.  Their run is cut off from its
+// first token on, every `most` of them, as far as the look back of 31 - most tokens reaches, there, and from there on where the token's
+// number is a multiple of `most`.
 // Asked by whole warps with the request of token `t + most - 1 - lane` (anything where there is no such token).
 // 0: token t is not the first of such a piece.
 __device__ __forceinline__ int run_of(const Batch& b, const Token& token, int t, int most, int seg_around) {
     if (!token.table) return 1;
     const int lane = threadIdx.x & 31, seg = __shfl_sync(0xffffffffu, seg_around, most - 1);
-    const int at = t + most - 1 - lane;
+    const int at = t + most - 1 - lane, reach = 31 - most;
     const unsigned same = __ballot_sync(0xffffffffu, at >= token.first && at < token.end && seg_around == seg);
-    int before = __ffs(~(same >> most)) - 1, inside = t - (32 - most);
-    for (bool more = before == 32 - most; more;) {
-        inside -= 32;
-        const int back = inside + 31 - lane;
-        const int n = __ffs(~__ballot_sync(0xffffffffu, back >= token.first && b.tok_seg[back] == seg)) - 1;
-        more = n < 0;                                      // all thirty-two
-        before += more ? 32 : n;
-    }
-    return before % most ? 0 : 1 + __clz(~(same << (33 - most)));
+    const int before = __ffs(~(same >> most)) - 1;         // tokens of the run in front of t, reach + 1 and more as reach + 1
+    const int behind = __clz(~(same << (33 - most)));      // and behind it, at most most - 1
+    // lane d: whether token t + d begins a piece (behind the run: as if)
+    const int offset = before + lane;
+    const bool begins = lane > behind || (offset <= reach ? offset == reach || offset % most == 0 : (t + lane) % most == 0);
+    const unsigned pieces = __ballot_sync(0xffffffffu, begins);
+    return pieces & 1 ? __ffs(pieces >> 1) : 0;
 }
 // 2^(m - of), 0 for a part that has seen nothing
 __device__ __forceinline__ float part_weight(float m, float of) { return m == -INFINITY ? 0.0f : ex2(m - of); }

@@ -11,6 +11,10 @@
 // Many rows: a warp has up to 2,048 columns of one, so that as much as possible is on the way at once and nobody waits at
 // a barrier; few: a block has a row, a thread eight columns, for the shortest way through.  Rounding by adding 1.5 * 2^23, whose
 // low byte is the integer: the conversion instructions have a quarter of the adders' rate.
+//
+// Measured on B200: 4,096 rows of 8,192 in bf16 19.0 us (100 MB: 5.3 TB/s, of 6.57 that a copy reaches; issue slots half busy),
+// 8,192 of 2,048 in fp32 15.8 (5.3 TB/s), with the norm and eight pieces a thread 21.5 (3.9 TB/s: a warp's registers leave
+// 28 % of the warps).
 #include "int8_quantize.cuh"
 
 using namespace fwb;
