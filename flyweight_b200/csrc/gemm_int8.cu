@@ -682,7 +682,7 @@ FWB_API int fwb_gemm_int8(const void* X, const float* xs, const void* W, const f
 }
 
 FWB_API int fwb_rows_int8(const void* x, int x_bf16, const float* delta, const float* norm_w, const int* rows, void* q,
-                          float* scales, int R, int K, int stride, float eps, cudaStream_t stream);
+                          float* scales, int R, int K, int stride, int x_rows, float eps, cudaStream_t stream);
 
 // The same for rows that are no integers yet: x [M][K] bf16 (x_bf16) or fp32; scratch: M * stride bytes for the integers and
 // 4 M behind them for the scales, stride = K rounded up to 16.  Without scratch (null): in one launch, for at most 8 tokens and 4,096
@@ -703,7 +703,7 @@ FWB_API int fwb_linear_int8(const void* x, int x_bf16, void* scratch, const void
         return few_raw_tokens(p, x, x_bf16 != 0, code, stream);
     }
     float* scales = reinterpret_cast<float*>(static_cast<char*>(scratch) + (size_t)M * stride);
-    const int status = fwb_rows_int8(x, x_bf16, nullptr, nullptr, nullptr, scratch, scales, M, K, stride, 0.0f, stream);
+    const int status = fwb_rows_int8(x, x_bf16, nullptr, nullptr, nullptr, scratch, scales, M, K, stride, M, 0.0f, stream);
     if (status != FWB_OK) return status;
     return fwb_gemm_int8(scratch, scales, W, ws, Y, addend, M, N, K, stride, w_stride, w_rows, epilogue, up_row_offset, gate_limit,
                          0, 1, stream);

@@ -31,7 +31,7 @@ struct RowsInt8Params {
     const int* rows;             // row indices or null
     signed char* q;              // [R][stride]
     float* scales;               // [R]
-    int R, K, stride;
+    int R, K, stride, x_rows;    // x_rows: rows that x has, for the indices
     float eps;
     int vector;                  // rows start on 16-byte borders and K is a multiple of 8
 };
@@ -110,7 +110,13 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : CHUNKS == 8 ? 256 : 10
     pdl_entry();
     const int r = WARP ? blockIdx.x * WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && r >= prm.R) return;
-    const T* row = reinterpret_cast<const T*>(prm.x) + (prm.rows ? (size_t)prm.rows[r] : (size_t)r) * K;
+    const int from = FORM == NORM && prm.rows ? prm.rows[r] : r;
+    if (FORM == NORM && (from < 0 || from >= prm.x_rows)) {            // no such row: zeros
+        for (int k = k0; k < prm.stride; k += step) *reinterpret_cast<uint2*>(prm.q + (size_t)r * prm.stride + k) = make_uint2(0, 0);
+        if (k0 == 0) prm.scales[r] = 0.0f;
+        return;
+    }
+    const T* row = reinterpret_cast<const T*>(prm.x) + (size_t)from * K;
     Raw<T> raw[HELD];
     if constexpr (CHUNKS > 0) {
 #pragma unroll
@@ -218,13 +224,15 @@ void launch(const RowsInt8Params& prm, cudaStream_t stream) {
 }  // namespace
 
 // x: [.][K] (row r, or rows[r]) in bf16 (x_bf16) or fp32; q: [R][stride] int8, stride >= K a multiple of 16; scales: [R].
-// norm_w: [K] or null; with it x is fp32, and delta [.][K] (or null) is added into x in place first.
+// norm_w: [K] or null; with it x is fp32, has x_rows rows (an index beyond them gives zeros), and delta [.][K] (or null) is added into
+// x in place first.
 FWB_API int fwb_rows_int8(const void* x, int x_bf16, const float* delta, const float* norm_w, const int* rows, void* q,
-                          float* scales, int R, int K, int stride, float eps, cudaStream_t stream) {
+                          float* scales, int R, int K, int stride, int x_rows, float eps, cudaStream_t stream) {
     if (R <= 0) return FWB_OK;
     if (!x || !q || !scales || K <= 0 || stride < K || (stride & 15) || ((uintptr_t)q & 15)) return FWB_BAD_ARGUMENT;
-    if ((delta && !norm_w) || (norm_w && x_bf16) || (delta && rows)) return FWB_UNSUPPORTED;
-    RowsInt8Params prm{x, delta, norm_w, rows, (signed char*)q, scales, R, K, stride, eps, 0};
+    if ((delta && !norm_w) || (norm_w && x_bf16) || (rows && (delta || !norm_w))) return FWB_UNSUPPORTED;
+    if (!rows && R > x_rows) return FWB_BAD_ARGUMENT;
+    RowsInt8Params prm{x, delta, norm_w, rows, (signed char*)q, scales, R, K, stride, x_rows, eps, 0};
     const uintptr_t bits = (uintptr_t)x | (uintptr_t)delta | (uintptr_t)norm_w;
     prm.vector = (K & 7) == 0 && (bits & 15) == 0;
     if (delta) launch<float, NORM_DELTA>(prm, stream);

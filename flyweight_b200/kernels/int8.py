@@ -94,7 +94,7 @@ def _quantize(x: torch.Tensor, is_bf16: int, delta, norm, rows, eps: float, kind
     R = rows.numel() if rows is not None else x.shape[0]
     made = kind(_scratch(R, K, x.device), R, K)
     lib.call("fwb_rows_int8", x.data_ptr(), is_bf16, lib.ptr(delta), lib.ptr(norm), lib.ptr(rows), made._address, made._scales, R, K,
-             made._stride, eps, lib.stream())
+             made._stride, x.shape[0], eps, lib.stream())
     return made
 
 
@@ -118,7 +118,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
                  rows: Optional[torch.Tensor] = None) -> Int8Rows:
     """``ops.rmsnorm`` whose rows leave as integers: ``(x / sqrt(mean(x^2) + eps)) * weight`` per row of the fp32 residual
     ``x``.  With ``delta`` the residual sum ``x += delta`` happens first, in place; with ``rows`` (int32) only those rows are
-    normalised, into compact rows (not together with ``delta``)."""
+    normalised, into compact rows (not together with ``delta``); an index that is no row of ``x`` gives a row of zeros."""
     if _input("residual", x):
         raise KernelError("the residual must be float32")
     check_tensor("norm weight", weight, _FP32, (x.shape[1],))

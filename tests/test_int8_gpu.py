@@ -170,6 +170,18 @@ def test_normed_rows_of_an_index():
     assert torch.equal(some.values, every.values[rows.long()]) and torch.equal(some.scales, every.scales[rows.long()])
 
 
+@pytest.mark.parametrize("R,K", [(4, 96), (5, 2047), (7, 20000), (2400, 300)])
+def test_an_index_that_is_no_row_gives_zeros(R, K):
+    from flyweight_b200.kernels import int8
+    x, w = rows_of(9, K, torch.float32).to(DEV), torch.ones(K, device=DEV)
+    rows = torch.arange(R, dtype=torch.int32) % 9
+    rows[1], rows[3] = -1, 9
+    some, every = int8.rmsnorm_int8(x, w, 1e-5, rows=rows.to(DEV)), int8.rmsnorm_int8(x, w, 1e-5)
+    there = [r for r in range(R) if r not in (1, 3)]
+    assert not some.values[[1, 3]].any() and not some.scales[[1, 3]].any()
+    assert torch.equal(some.float()[there], every.float()[rows[there].long().to(DEV)])
+
+
 # tokens, columns, features: one token to a prompt, sizes that fill no tile on either side of every choice of kernel
 PRODUCTS = [(1, 16, 8), (1, 2048, 2048), (2, 100, 33), (3, 4097, 130), (7, 1, 5), (8, 2048, 1024), (9, 640, 257), (16, 1024, 4608),
             (17, 512, 129), (24, 96, 300), (31, 1040, 1000), (33, 200, 64), (64, 4096, 512), (65, 129, 260), (100, 48, 1),
