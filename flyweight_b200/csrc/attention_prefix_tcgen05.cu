@@ -175,14 +175,24 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();                  // q, the pages and the batch's arrays come from earlier in the stream
-    pdl_launch_dependents();     // (only now: the own kernel goes by everything in front of this one being done)
+    // Tensor memory is this CTA's before a kernel behind may start: one behind the own kernel could else take the columns and hold
+    // them while it waits, by way of the own kernel, for this one.  (Not ahead of the wait: the same of the kernel in front.)
+    if (warp == 1) tmem_alloc(tmem_holder, L::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_holder;
+    pdl_launch_dependents();     // (only now, too: the own kernel goes by everything in front of this one being done)
 
     // every warp finds the work by itself: the tile's tokens, its slice of the pages, how far anybody sees
     const int per_tile = ROWS / prm.head_chunk;
     const TokenTile tile = token_tile(prm.b, blockIdx.x, per_tile);
     const int pages = tile.pages, per = pages_per_slice(pages, prm.splits);
     const int page0 = blockIdx.z * per, page1 = min(pages, page0 + per);
-    if (page0 >= page1) return;                            // (the whole CTA: nobody has allocated or asked for anything)
+    if (page0 >= page1) {                                  // (the whole CTA: nobody has asked for anything)
+        if (warp == 1) tmem_dealloc(tmem_base, L::TMEM_COLS);
+        return;
+    }
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
     const int* table = prm.b.row_of(tile.group_first);
@@ -192,12 +202,6 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     far = min(__reduce_max_sync(0xffffffffu, far), page1 * KEYS - 1);
     const int n_pages = !table || far < page0 * KEYS ? 0 : far / KEYS + 1 - page0;
     const int n_steps = (n_pages + PAGES - 1) / PAGES;
-
-    if (warp == 1) tmem_alloc(tmem_holder, L::TMEM_COLS);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_holder;
     int asked = 0;                                         // the producer's: steps asked for so far
 
     if (warp == 0) {
