@@ -94,7 +94,6 @@ gemm_int8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     float* x_scale = reinterpret_cast<float*>(tiles + T::data_bytes(STAGES, splits) + 256);     // [BN]
 
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tok0 = blockIdx.x * BN, feat0 = blockIdx.y * BM;
     const int kb_begin = blockIdx.z * prm.kb_per_split;
@@ -114,6 +113,7 @@ gemm_int8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();     // (only with tensor memory in hand: a kernel further back could hold the columns and wait for this one)
     const uint32_t tmem_base = *tmem_holder;
     int asked = 0;                                     // the producer's: stages filled so far
 
@@ -357,7 +357,6 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();                // 0 = leader
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1, n_kb = prm.n_kb;
@@ -383,6 +382,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __syncthreads();
     cluster_sync_all();          // both CTAs' barriers exist before anybody signals across
     tc_fence_after();
+    pdl_launch_dependents();     // (only with tensor memory in hand, as above)
     const uint32_t tmem_base = *tmem_holder;
 
     int asked = 0;                                       // the producer's: stages filled so far

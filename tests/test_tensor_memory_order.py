@@ -33,7 +33,8 @@ def lets_go_too_early(body):
     return bool(alloc and go and go.start() < alloc.start())
 
 
-@pytest.mark.parametrize("source,names", [("attention_prefix_tcgen05.cu", {"prefix_tcgen05_kernel"})])
+@pytest.mark.parametrize("source,names", [("attention_prefix_tcgen05.cu", {"prefix_tcgen05_kernel"}),
+                                          ("gemm_int8.cu", {"gemm_int8_tile_kernel", "gemm_int8_pair_kernel"})])
 def test_tensor_memory_comes_before_the_next_kernel(source, names):
     bodies = kernels((CSRC / source).read_text())
     assert {name for name, body in bodies.items() if ALLOC.search(body)} == names
