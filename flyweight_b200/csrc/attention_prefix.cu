@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
     for (int i = 0; i < 4; ++i) {
         const int r = ty * 4 + i, tok = r / prm.head_chunk;
         const bool is_row = tok < tile.count && r % prm.head_chunk < heads;
-        last[i] = is_row && prm.b.row_of(tile.first + tok) ? prm.b.positions[tile.first + tok] : -1;
+        last[i] = is_row && prm.b.row_of(tile.first + tok) ? prm.b.last_key(prm.b.positions[tile.first + tok]) : -1;
         if (is_row) whole_to = min(whole_to, last[i]);
     }
     float m[4], l[4], acc[4][COLS][4];

@@ -34,8 +34,10 @@ struct Batch {
         const int seg = tok_seg[token];
         return seg < 0 || seg >= n_segments ? nullptr : block_table + (size_t)seg * max_pages;
     }
-    // the last key that a token at this position sees
-    __device__ __forceinline__ int last_key(int position) const { return position < max_pages * PAGE ? position : max_pages * PAGE - 1; }
+    // the last key that a token at this position sees: -1 (none) in front of the first one, wherever
+    __device__ __forceinline__ int last_key(int position) const {
+        return position < 0 ? -1 : position < max_pages * PAGE ? position : max_pages * PAGE - 1;
+    }
     __device__ __forceinline__ bool is_page(int page) const { return page >= 0 && page < num_pages; }
 };
 

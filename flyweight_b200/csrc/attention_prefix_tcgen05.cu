@@ -198,7 +198,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int* table = prm.b.row_of(tile.group_first);
     int far = -1;
     for (int i = lane; i < tile.count; i += 32)
-        if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.positions[tile.first + i]);
+        if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.last_key(prm.b.positions[tile.first + i]));
     far = min(__reduce_max_sync(0xffffffffu, far), page1 * KEYS - 1);
     const int n_pages = !table || far < page0 * KEYS ? 0 : far / KEYS + 1 - page0;
     const int n_steps = (n_pages + PAGES - 1) / PAGES;
@@ -284,7 +284,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int t_in = row / prm.head_chunk, h_in = row - t_in * prm.head_chunk;
         const bool valid = t_in < tile.count && h_in < heads;
         const int tok = tile.first + (valid ? t_in : 0), head = kvh * prm.group + head0 + (valid ? h_in : 0);
-        const int hi = min(far, valid && prm.b.row_of(tok) ? prm.b.positions[tok] : -1);
+        const int hi = min(far, valid && prm.b.row_of(tok) ? prm.b.last_key(prm.b.positions[tok]) : -1);
         float m = -INFINITY, l = 0.0f;
         if (n_steps > 0) {
             const __nv_bfloat16* q_row = prm.q + ((size_t)tok * prm.nh + head) * prm.hd;
@@ -298,7 +298,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (lane == 0) mbar_arrive(q_ready);
         }
         // from which key on some row of this warp does not see everything, and whether all of the slice's pages are pages
-        const int whole_to = (int)__reduce_min_sync(0xffffffffu, (unsigned)(valid ? hi + 1 : 0x7fffffff));
+        const int whole_to = __reduce_min_sync(0xffffffffu, valid ? hi + 1 : 0x7fffffff);
         bool all_pages = true;
         for (int i = lane; i < n_pages; i += 32) all_pages &= prm.b.is_page(table[page0 + i]);
         all_pages = __all_sync(0xffffffffu, all_pages);

@@ -348,3 +348,31 @@ def test_refusals():
             attention.shared_prefix_attention(**{**good, **more})
     with pytest.raises(KernelError):
         attention.shared_prefix_attention(**wide)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("position", [-1, -2, -64, -2 ** 31])
+def test_a_token_before_the_first_key_sees_nothing(cut, neighbours, dtype, dim, position):
+    """Among tokens that see all of the shared pages, so that no other row of the block needs a mask."""
+    case = Case([(18, [(1, 10 + i) for i in range(12)]), (2, [(3, 70)])], 8, 2, dim, dtype)
+    for token in (0, 5, 11, 13):
+        case.positions[token] = position
+    case.check(attend(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("position", [-1, -2, -2 ** 31])
+def test_a_token_before_the_first_key_takes_nothing_from_its_neighbours(cut, neighbours, dtype, dim, position):
+    """Infinities and NaN in the last key and value of the token's own request, which another of its tokens sees."""
+    case = Case([(18, [(3, 40), (1, 7), (5, 66)])], 6, 2, dim, dtype)
+    case.positions[0] = case.positions[5] = position
+    want = attend(case).clone()
+    for row, n in zip((0, 2), (18 * 64 + 40, 18 * 64 + 66)):
+        page = case.rows[row][(n - 1) // PAGE]
+        case.k[page, :, (n - 1) % PAGE], case.v[page, :, (n - 1) % PAGE] = math.nan, math.inf
+    got = attend(case)
+    seen = [0, 1, 3, 4, 5, 6, 7]
+    assert not got[[0, 5]].any() and torch.equal(got[seen], want[seen])
+    assert torch.isnan(got[[2, 8]].float()).all()
