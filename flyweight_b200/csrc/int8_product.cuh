@@ -33,7 +33,12 @@ __device__ __forceinline__ void store(const Product& p, size_t at, float v, floa
     if (EPI == EPI_F32) reinterpret_cast<float*>(p.y)[at] = v;
     else if (EPI == EPI_BF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
     else if (EPI == EPI_ADD_F32) reinterpret_cast<float*>(p.y)[at] = __fadd_rn(v, add);
-    else reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(tc5::gated_fast(p.act, p.limit, v, u));
+    else {
+        float y = tc5::gated_fast(p.act, p.limit, v, u);
+        // a row or feature of the scale NaN: these two cut off by minima and maxima, which take the number beside a NaN
+        if ((p.act == tc5::GATE_SWISH_CLAMPED || p.act == tc5::GATE_RELU) && (v != v || u != u)) y = __int_as_float(0x7fffffff);
+        reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(y);
+    }
 }
 
 // The product of a few tokens (host function, linear_rows_int8.cu); at most MAX_FEW of them.

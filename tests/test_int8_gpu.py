@@ -367,3 +367,24 @@ def test_refusals():
                                            rows=torch.zeros(1, dtype=torch.int32, device=DEV))):
         with pytest.raises(KernelError):
             call()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "relu", "swish_clamped"])
+@pytest.mark.parametrize("M,form", [(7, None), (7, (8, 1)), (7, (32, 1)), (30, (8, 1)), (30, (32, 2)), (70, (64, 1)), (70, (64, 4)), (70, (128, 2)),
+                                    (70, (-128, 1)), (300, (-256, 1))])
+def test_nan_stays_nan_behind_every_gate(M, form, act):
+    """A row with an infinity or NaN, and a feature whose gate or up weights hold one: NaN in all that is made of them, whatever the
+    activation cuts off, and nowhere else.  ``form`` None: the integers are made inside the product."""
+    from flyweight_b200.kernels import int8, ops
+    K, F, limit = 512, 260, 3.0
+    x, w = rows_of(M, K, torch.bfloat16, 1), rows_of(2 * F, K, torch.bfloat16, 2) * K ** -0.5
+    x[2, 0], x[4, K - 1], w[9, 3], w[F + 130, 7], w[F - 1, 0] = math.nan, -math.inf, math.nan, math.inf, -math.inf
+    nan = torch.zeros(M, F, dtype=torch.bool)
+    nan[[2, 4]], nan[:, [9, 130, F - 1]] = True, True
+    matrix, x = int8.matrix_int8(w.to(DEV)), x.to(DEV)
+    if form is None:
+        got = int8.gated_int8(x, matrix, activation=act, limit=limit)
+    else:
+        got = torch.empty((M, F), dtype=torch.bfloat16, device=DEV)
+        int8._product(int8.rows_int8(x), matrix, got, None, F, 3 | ops.GATE_ACTIVATIONS[act] << 8, limit, *form)
+    assert torch.equal(torch.isnan(got).cpu(), nan) and torch.isfinite(got.cpu()[~nan]).all()
