@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(THREADS) prefix_kernel(const Params prm) {
     if (page0 >= page1) return;
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
-    const int* table = prm.b.row_of(tile.group_first);
+    const int* table = shared_row(prm.b, tile);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, rows = tile.count * prm.head_chunk;
     const bool works = (threadIdx.x >> 5) * 8 < rows;  // a warp has eight rows; those without any only fetch
 

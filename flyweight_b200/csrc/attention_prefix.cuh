@@ -1,8 +1,8 @@
 // What the kernels of attention over a shared prefix have in common: the batch as they see it.
 //
 // The tokens [group_start[g], group_start[g + 1]) belong to requests whose first group_pages[g] pages are the same ones;
-// the group's first token's block-table row names them.  A token sees the keys up to its own position: those of the shared
-// pages, then its request's own from position 64 * group_pages[g] on.
+// the block-table row of the group's first token that belongs to a request names them.  A token sees the keys up to its own
+// position: those of the shared pages, then its request's own from position 64 * group_pages[g] on.
 #pragma once
 
 #include "common.cuh"
@@ -41,10 +41,10 @@ struct Batch {
     __device__ __forceinline__ bool is_page(int page) const { return page >= 0 && page < num_pages; }
 };
 
-// The token tile `index` when every group's tokens are cut into tiles of `per_tile`: its group's first token and pages, its own
+// The token tile `index` when every group's tokens are cut into tiles of `per_tile`: its group's tokens and pages, its own
 // first token and tokens (0: no such tile).  Asked by whole warps; everything it reads is asked for at once.
 struct TokenTile {
-    int group_first, pages, first, count;
+    int group_first, group_end, pages, first, count;
 };
 __device__ __forceinline__ TokenTile token_tile(const Batch& b, int index, int per_tile) {
     const int lane = threadIdx.x & 31;
@@ -67,14 +67,25 @@ __device__ __forceinline__ TokenTile token_tile(const Batch& b, int index, int p
             TokenTile t;
             t.group_first = __shfl_sync(0xffffffffu, first, owner);
             t.pages = __shfl_sync(0xffffffffu, pages, owner);
+            t.group_end = t.group_first + __shfl_sync(0xffffffffu, n, owner);
             t.first = t.group_first + inside * per_tile;
-            const int left = __shfl_sync(0xffffffffu, n, owner) - inside * per_tile;
+            const int left = t.group_end - t.first;
             t.count = left < per_tile ? left : per_tile;
             return t;
         }
         index -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    return TokenTile{0, 0, 0, 0};
+    return TokenTile{0, 0, 0, 0, 0};
+}
+// The block-table row that names the shared pages of a tile's group (null: none of its tokens belongs to a request).  Asked by whole warps.
+__device__ __forceinline__ const int* shared_row(const Batch& b, const TokenTile& tile) {
+    const int lane = threadIdx.x & 31;
+    for (int t0 = tile.group_first; t0 < tile.group_end; t0 += 32) {
+        const int seg = t0 + lane < tile.group_end ? b.tok_seg[t0 + lane] : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, seg >= 0 && seg < b.n_segments);
+        if (there) return b.block_table + (size_t)__shfl_sync(0xffffffffu, seg, __ffs(there) - 1) * b.max_pages;
+    }
+    return nullptr;
 }
 // The most such tiles a batch can have, from what the host knows.
 inline long most_token_tiles(int T, int n_groups, int per_tile) {

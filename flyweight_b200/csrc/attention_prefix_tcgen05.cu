@@ -195,7 +195,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     const int kvh = blockIdx.y / prm.head_chunks, head0 = (blockIdx.y % prm.head_chunks) * prm.head_chunk;
     const int heads = min(prm.head_chunk, prm.group - head0);
-    const int* table = prm.b.row_of(tile.group_first);
+    const int* table = shared_row(prm.b, tile);
     int far = -1;
     for (int i = lane; i < tile.count; i += 32)
         if (prm.b.row_of(tile.first + i)) far = max(far, prm.b.last_key(prm.b.positions[tile.first + i]));

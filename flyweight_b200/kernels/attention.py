@@ -334,7 +334,8 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     ``q`` [T][n_heads * head_dim], the pools [pages][kv_heads][64][head_dim] (all bf16 or all fp32), ``positions`` and
     ``tok_seg`` [T], ``block_table`` [requests][pages] as in ``paged_attention``.  The tokens ``group_start[g]`` to
     ``group_start[g + 1]`` (int32 [groups + 1], rising) are group g's; the block-table rows of its requests begin with the same
-    ``group_pages[g]`` pages (int32 [groups]; 0: nothing shared), named by the row of its first token.  Every token sees
+    ``group_pages[g]`` pages (int32 [groups]; 0: nothing shared), named by the row of its first token that belongs to a request
+    (one whose ``tok_seg`` is a row of the table; the others get zeros).  Every token sees
     the keys up to its position, in shared and own pages alike, whatever the number of tokens a request has in the step; the
     result is ``paged_attention``'s.  Shared values that one of a group's tokens sees must be finite.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
     position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are in ``out``.

@@ -376,3 +376,19 @@ def test_a_token_before_the_first_key_takes_nothing_from_its_neighbours(cut, nei
     seen = [0, 1, 3, 4, 5, 6, 7]
     assert not got[[0, 5]].any() and torch.equal(got[seen], want[seen])
     assert torch.isnan(got[[2, 8]].float()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("leading", [1, 3, 35])
+def test_a_group_led_by_tokens_of_no_request(cut, neighbours, dtype, dim, leading):
+    """Finished slots stay in a batch as tokens of no request: they get zeros, and the others of the group see what they saw."""
+    from flyweight_b200.kernels import attention
+    case = Case([(9, [(1, 10 + i) for i in range(leading + 2)]), (2, [(3, 70), (1, 5)]), (3, [(1, 9)])], 8, 4, dim, dtype)
+    d = case.device()
+    gone = list(range(leading)) + [leading + 2, leading + 6]       # ... the second group's first token, all of the third group's
+    d["tok_seg"][gone] = torch.tensor([-1, len(case.rows)], dtype=torch.int32, device=DEV).repeat(len(gone))[:len(gone)]
+    got = attention.shared_prefix_attention(**d)
+    for token in gone:
+        case.positions[token] = -1
+    case.check(got)
