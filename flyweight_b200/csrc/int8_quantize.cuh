@@ -11,7 +11,9 @@ namespace fwb {
 namespace int8 {
 
 constexpr int CHUNK = 8;                 // elements a thread takes at once
-constexpr float TINY_ROW = 1e-30f;       // a row without a larger value is taken as zeros: its scale would be no normal number
+// A row of smaller values alone is taken as zeros: 127 * 2^-125, from where on half of the scale is a normal number and so every
+// remainder beside it exact.
+constexpr float TINY_ROW = 0x1.fcp-119f;
 
 struct RowScale {
     float stored;                // what goes with the row

@@ -100,8 +100,8 @@ def _quantize(x: torch.Tensor, is_bf16: int, delta, norm, rows, eps: float, kind
 
 def rows_int8(x: torch.Tensor) -> Int8Rows:
     """Every row of ``x`` ([R][K], bf16 or fp32) as integers of [-127, 127]: ``scale = max|x| / 127`` in fp32,
-    ``value = round(x / scale)``, ties to even.  A row of zeros (nothing from 1e-30 on) has the scale 0; a row with an infinity
-    or a NaN has the scale NaN."""
+    ``value = round(x / scale)``, ties to even.  A row of zeros (nothing from 127 * 2^-125 = 3e-36 on) has the scale 0; a row
+    with an infinity or a NaN has the scale NaN, and what is made of it is NaN."""
     return _quantize(x, _input("rows", x), None, None, None, 0.0, Int8Rows)
 
 

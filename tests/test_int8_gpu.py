@@ -388,3 +388,30 @@ def test_nan_stays_nan_behind_every_gate(M, form, act):
         got = torch.empty((M, F), dtype=torch.bfloat16, device=DEV)
         int8._product(int8.rows_int8(x), matrix, got, None, F, 3 | ops.GATE_ACTIVATIONS[act] << 8, limit, *form)
     assert torch.equal(torch.isnan(got).cpu(), nan) and torch.isfinite(got.cpu()[~nan]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [64, 520, 9000])
+def test_small_rows_become_the_defined_integers(K, dtype):
+    """Down to rows whose largest value is 127 * 2^-125, so that half of the scale is a normal number; smaller rows are zeros."""
+    from flyweight_b200.kernels import int8
+    least = 127 * 2.0 ** -125
+    tops = torch.tensor([1e-28, 1.1e-30, 9e-31, 3e-33, 1e-35, 3 * least, least * (1 + 2.0 ** -7), least], dtype=F64)
+    g = torch.Generator().manual_seed(7)
+    x = (torch.rand(len(tops), K, generator=g, dtype=F64) * 2 - 1) * tops[:, None]
+    x[:, 5] = tops
+    if dtype == torch.float32:                       # values on and next to every half
+        scale = (tops.to(dtype).to(F64) / 127).to(dtype).to(F64)
+        halves = (torch.arange(40).to(F64) + 0.5) * scale[:, None]
+        x[:, 6:46] = halves * (1 + torch.tensor([0.0, 2.0 ** -23, -2.0 ** -23, 2.0 ** -22]).to(F64).repeat(10))
+    x = x.to(dtype)
+    assert (x.to(F64).abs().amax(dim=1) >= least).all()
+    for rows in (x, x.repeat(400, 1)):               # the forms that few and many rows take
+        values, scale = define(rows)
+        got = int8.rows_int8(rows.to(DEV))
+        assert torch.equal(got.scales.cpu(), scale) and torch.equal(got.values[:, :K].cpu().to(F64), values)
+    below = torch.full((3, K), least * (1 - 2.0 ** -8), dtype=F64).to(dtype)
+    below[1:] *= 2.0 ** -10
+    below[2, 1:] = 0
+    got = int8.rows_int8(below.to(DEV))
+    assert not got.values.any() and not got.scales.any()
