@@ -356,7 +356,7 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     check_tensor("k pool", k_pool, dtype)
     check_tensor("v pool", v_pool, dtype, k_pool.shape)
     num_pages, n_kv, _, head_dim = k_pool.shape
-    if n_heads <= 0 or n_heads % n_kv or columns != n_heads * head_dim:
+    if n_heads <= 0 or n_kv == 0 or n_heads % n_kv or columns != n_heads * head_dim:
         raise KernelError(f"q has {columns} columns, expected {n_heads} heads of {head_dim} over {n_kv} KV heads")
     if head_dim > 256:
         raise KernelError(f"head sizes up to 256, got {head_dim}")

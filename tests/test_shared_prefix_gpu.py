@@ -392,3 +392,12 @@ def test_a_group_led_by_tokens_of_no_request(cut, neighbours, dtype, dim, leadin
     for token in gone:
         case.positions[token] = -1
     case.check(got)
+
+
+@pytest.mark.parametrize("kv,dim", [(0, 64), (2, 0), (0, 0)])
+def test_pools_without_heads_are_refused(kv, dim):
+    from flyweight_b200.kernels import KernelError
+    case = Case(BATCHES["two"], 4, 2, 64, torch.bfloat16)
+    pool = torch.zeros(5, kv, 64, dim, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(KernelError):
+        attend(case, k_pool=pool, v_pool=pool, q=torch.zeros(2, 4 * dim, dtype=torch.bfloat16, device=DEV), out=None)
