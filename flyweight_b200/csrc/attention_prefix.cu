@@ -9,9 +9,10 @@
 // Masked keys are left out by selection, so neither infinities nor NaN in them reach a result; rows of V behind a request's last key
 // are not read.  A row that sees no key is zero.
 //
-// Bound by the latency of few blocks and the multiply-adds' issue: two groups of ten requests behind 1,024 keys, 10 heads over 5 of 80, capped
-// scores, fp32: 25 us on B200, 8 MB (0.3 TB/s).  64 rows a block, four by four scores a thread: a warp whose eight rows nobody has
-// only fetches.
+// Two groups of ten requests behind 1,024 keys, 10 heads over 5 of 80, capped scores, fp32: 25 us on B200, 8 MB (0.3 TB/s).  Neither memory
+// nor the multiply-adds bound it.  64 rows a block, four by four scores a thread, a warp whose eight rows nobody has only fetches:
+// ten tokens of two heads are 20 rows, so three of eight warps compute.  The own kernel is 100 blocks, which take their pages one
+// after the other, copies, scores, softmax and values each behind a barrier with nothing of the next page on the way.
 #include "attention_prefix.cuh"
 
 using namespace fwb;

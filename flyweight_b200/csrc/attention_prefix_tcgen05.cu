@@ -17,11 +17,12 @@
 // kernel reads before the join was written earlier than that.
 //
 // Measured on B200, bf16 (us; what the bytes take at a copy's 6.57 TB/s, the products at 1,670 TFLOP/s): 64 requests of 32 heads over 8
-// of 64 behind 8,192 keys, each with up to 500 of its own, 32.8 (7.8; 2.7): the prefix kernel 21.5, then 8 to 9 until the
+// of 64 behind 8,192 keys, each with up to 500 of its own, 31.7 (7.8; 2.7): the prefix kernel 21.5, then 8 to 9 until the
 // last own keys are walked and all is joined -- blocks' latencies from arrays to pages to products, 1.5 us a page under load;
-// 256 requests behind 32,768 keys, up to 1,000 own, 178 (50.5; 41.8): 120 and 58.  The prefix kernel there is bound by what the
-// softmax issues -- the special-function pipe is 56 % busy, the tensor pipe 39 %, DRAM 5 % -- with two warps a scheduler; the own kernel reads 290 MB at 5 TB/s, four CTAs an SM.  Two prefix CTAs an SM (82 or
-// 96 KiB each, 168 registers a thread) hide one's softmax behind the other's products; three with the scores under P: slower.
+// 256 requests behind 32,768 keys, up to 1,000 own, 175 (50.5; 41.8): 120 and 55, one behind the other.  In the prefix kernel there no
+// pipe is full -- special functions 56 %, tensor 39 %, issue slots 33 %, DRAM 5 % -- the two warps a scheduler wait along the chain of
+// scores, softmax and product; the own kernel reads 290 MB at 5 TB/s, four CTAs an SM.  Two prefix CTAs an SM (82 or 96 KiB each, 168
+// registers a thread) hide one's softmax behind the other's products; three with the scores under P: slower.
 //
 // Masked keys are left out by selection; rows of V behind the last key anybody sees are cleared in shared memory, so that
 // 0 * (infinity or NaN) cannot reach a result.  A page id outside the pool is fetched as zeros and masked.

@@ -15,10 +15,11 @@
 //                 form a cluster and add their accumulators through distributed shared memory
 //   pair kernel   CTA pairs (cta_group::2): 256 features (128 with a gate) x 256 or 128 tokens, persistent, two accumulators
 //
-// Measured on B200 (a copy reaches 6.57 TB/s; the bfloat16 tensor rate of 1,670 TFLOP/s twice over would be 3,340): pairs, 4096 x 8192 x 2048
-// 52 us (2,650 TOPS), gated 8192 x 2048 x 8192 232 us (2,370 TOPS) -- bound by what L2 hands out, 2.44 GB in all, 10 TB/s; the tensor
-// pipe is 62 % busy.  Tiles with slices, 64 x 8192 x 2048 10.9 us (1.6 TB/s; with the rows' launch 13.7), 333 x 1500 x 2047 with the rows'
-// launch 10.2: the latency of a walk over K (0.36 us a block of 128 k), of the cluster's join and of the launches.
+// Measured on B200 (a copy reaches 6.57 TB/s; the bfloat16 tensor rate of 1,670 TFLOP/s twice over would be 3,340): pairs, 4096 x 8192 x
+// 2048 52 us (2,650 TOPS): 128 tiles on 74 pairs are two rounds, the second with 54 pairs at work, which alone leaves 0.865 of the rate;
+// gated 8192 x 2048 x 8192 232 us (2,370 TOPS), bound by what L2 hands out, 2.44 GB in all, 10 TB/s; the tensor pipe is 62 % busy.
+// Tiles with slices, 64 x 8192 x 2048 10.2 us (1.6 TB/s; with the rows' launch 13.6), 333 x 1500 x 2047 with the rows' launch 10.1: the
+// latency of a walk over K (0.36 us a block of 128 k), of the cluster's join and of the launches.
 //
 // Launched with programmatic stream serialisation: the first ring of weights is asked for while the kernel in front still
 // runs.  Every wait on an mbarrier is bounded; after the limit the library's status word is raised, every role stops waiting,
@@ -65,12 +66,15 @@ __device__ __forceinline__ void drain(uint64_t* full_bar, int stages, int asked)
 }
 
 // ------------------------------------------------------------------ tile kernel
+// Stages of the ring, at most.  Measured on B200, us of the product with 2 3 4 5 6 8 stages: 64 x 8192 x 2048 in 32-token tiles and four
+// slices 13.3 10.9 10.2 10.2 10.8 11.0, in one 36.1 26.3 25.8 25.8 25.6 25.6; 333 x 1500 x 2047 8.6 7.5 7.4 7.2 7.3 7.5; gated 64 x 2048 x
+// 8192 15.6 13.7 13.4 13.6 13.6 13.6.  What a block of K takes is a latency that more bytes on the way do not hide.
+constexpr int RING = 4;
 template <int BN, int NACC>
 struct Tile {
     static constexpr int EPI_WARPS = BN >= 128 ? 16 : BN >= 64 ? 8 : 4;
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int STAGE_BYTES = NACC * A_BYTES + BN * BK8;
-    static constexpr int MAX_STAGES = 200 * 1024 / STAGE_BYTES > 8 ? 8 : 200 * 1024 / STAGE_BYTES;
     static constexpr int COLS = BN * NACC;
     static constexpr int TMEM_COLS = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
     static constexpr int PARTIAL_BYTES = COLS * BM * 4;
@@ -88,8 +92,8 @@ gemm_int8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int STAGES = prm.stages, splits = gridDim.z;
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + T::data_bytes(STAGES, splits));
-    uint64_t* empty_bar = full_bar + T::MAX_STAGES;
-    uint64_t* acc_bar = empty_bar + T::MAX_STAGES;
+    uint64_t* empty_bar = full_bar + RING;
+    uint64_t* acc_bar = empty_bar + RING;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     float* x_scale = reinterpret_cast<float*>(tiles + T::data_bytes(STAGES, splits) + 256);     // [BN]
@@ -265,7 +269,7 @@ int launch_tile(const CUtensorMap& map_w, const CUtensorMap& map_x, Params prm, 
     using T = Tile<BN, EPI == EPI_GATED_BF16 ? 2 : 1>;
     auto kernel = gemm_int8_tile_kernel<BN, EPI>;
     prm.kb_per_split = (prm.n_kb + splits - 1) / splits;
-    prm.stages = prm.kb_per_split < 4 ? prm.kb_per_split : 4;
+    prm.stages = prm.kb_per_split < RING ? prm.kb_per_split : RING;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
@@ -626,7 +630,7 @@ void choose(int M, int N, int K, bool gated, int* tile, int* splits) {
         for (int s = 1; s <= 8 && (s == 1 || n_kb >= 2 * s); s *= 2) {
             const long ctas = (long)((N + BM - 1) / BM) * ((M + t - 1) / t) * s;
             // CTAs the SMs hold at once, by shared memory; clusters leave SMs of a GPC over, and beyond that would wait for one another
-            const int kb = (n_kb + s - 1) / s, ring = (kb < 4 ? kb : 4) * (halves * A_BYTES + t * BK8), sums = s > 1 ? halves * t * BM * 4 : 0;
+            const int kb = (n_kb + s - 1) / s, ring = (kb < RING ? kb : RING) * (halves * A_BYTES + t * BK8), sums = s > 1 ? halves * t * BM * 4 : 0;
             const long held = (s > 1 && t == 128 ? 1 : 227 * 1024 / ((ring > sums ? ring : sums) + 2048)) * (s > 1 ? SM_COUNT * 7 / 8 : SM_COUNT);
             if (s > 1 && ctas > (held < 2 * SM_COUNT * 7 / 8 ? held : 2 * SM_COUNT * 7 / 8)) continue;
             const bool crowded = ctas > SM_COUNT && ctas <= held;

@@ -41,9 +41,11 @@ __device__ __forceinline__ RowScale row_scale(unsigned top, bool short_values) {
 // Checked: n = x (1 / s) rounded is the integer or its neighbour; e = x - n s has no rounding error (a multiple of the smaller
 // of x's and s's last places, and at most about s / 2), so |e| against s / 2 tells.
 //
-// Not checked, for values of eight bits under a maximum m of eight bits (bfloat16 rows): 254 |x| / m is an odd integer, and x / (m / 127)
-// a tie, or it is 2^-8 or more away from one.  s is m / 127 rounded, so the ties all lie on one side of their halves, by 2^-24 of
-// themselves at most; `inv` is 1 / s moved by 2^-22 of itself towards that side, which decides every tie and nothing else.
+// Not checked, for values of eight bits under a maximum m of eight bits (bfloat16 rows): with x = a 2^i, m = b 2^j and whole a, b below 256,
+// i <= j, the quotient x / (m / 127) is a tie where 254 a = (2 n + 1) b 2^(j - i), and else the two sides, whole numbers, differ by 1 or
+// more: the quotient is 1 / (254 a) of itself, more than 2^-16, away from a tie.  s is m / 127 rounded, so the ties all lie on one side of
+// their halves, by 2^-24 of themselves at most; `inv` is 1 / s moved by 2^-22 of itself towards that side (with the roundings of s, of
+// 1 / s and of the move less than 2^-21 in all), which decides every tie and nothing else.
 template <bool CHECKED>
 __device__ __forceinline__ uint2 quantize_by(const float (&v)[CHUNK], float s, float inv) {
     constexpr float ROUND = 12582912.0f;               // 1.5 * 2^23

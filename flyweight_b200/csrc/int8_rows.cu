@@ -13,8 +13,8 @@
 // low byte is the integer: the conversion instructions have a quarter of the adders' rate.
 //
 // Measured on B200: 4,096 rows of 8,192 in bf16 19.0 us (100 MB: 5.3 TB/s, of 6.57 that a copy reaches; issue slots half busy),
-// 8,192 of 2,048 in fp32 15.8 (5.3 TB/s), with the norm and eight pieces a thread 21.5 (3.9 TB/s: a warp's registers leave
-// 28 % of the warps).
+// 8,192 of 2,048 in fp32 15.8 (5.3 TB/s), with the norm and eight pieces a thread 21.5 (3.9 TB/s: the registers of a warp that holds
+// a whole row leave 28 % of the warps).
 #include "int8_quantize.cuh"
 
 using namespace fwb;
@@ -206,7 +206,10 @@ void launch(const RowsInt8Params& prm, int threads, cudaStream_t stream) {
     fwb::pdl(rows_int8_kernel<T, FORM, WARP, CHUNKS>, WARP ? (prm.R + WARP_ROWS - 1) / WARP_ROWS : prm.R, threads, 0, stream)(prm);
 }
 
-// (2,048 columns of bf16, us: 1,000 rows by blocks 3.4; 1,200 rows by warps 5.5; 8,192 rows by warps 15.2, by blocks 22)
+// Measured on B200 (us, by blocks and by warps; 1,000 2,368 4,000 6,000 8,192 rows): 1,024 columns of bf16 2.2 2.7, 3.4 3.0, 4.5 4.4, 6.6 4.9,
+// 9.1 5.7, of fp32 2.6 3.1, 3.7 4.5, 5.0 5.3, 6.8 6.1, 9.2 7.2; 2,048 of bf16 2.7 4.5, 4.7 4.8, 6.8 6.9, 9.5 8.6, 12.2 10.4, of fp32 3.3 4.6,
+// 5.4 6.5, 7.9 9.9, 11.2 12.8, 15.2 15.8, behind a norm 4.8 6.8, 8.5 8.6, 12.5 13.8, 17.9 17.6, 23.4 22.3.  The two change places between
+// 2,368 rows (where a warp a row fills the SMs) and 6,000; in between this border costs up to 2 us.
 constexpr int MANY_ROWS = 148 * 16;
 template <typename T, int FORM>
 void launch(const RowsInt8Params& prm, cudaStream_t stream) {

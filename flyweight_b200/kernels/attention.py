@@ -337,9 +337,10 @@ def shared_prefix_attention(q, k_pool, v_pool, positions, tok_seg, block_table, 
     ``group_pages[g]`` pages (int32 [groups]; 0: nothing shared), named by the row of its first token that belongs to a request
     (one whose ``tok_seg`` is a row of the table; the others get zeros).  Every token sees
     the keys up to its position, in shared and own pages alike, whatever the number of tokens a request has in the step; the
-    result is ``paged_attention``'s.  Shared values that one of a group's tokens sees must be finite.  A page id outside the pool is not read: its keys are not seen.  A token at a negative
-    position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are in ``out``.
-    ``scale`` is positive.
+    result is ``paged_attention``'s without a window: ``window`` and ``keep_first`` are not here, so layers that have them keep that one.
+    Shared values that one of a group's tokens sees must be finite.  A page id outside the pool is not read: its keys are not seen.
+    A token at a negative position sees nothing and gets zeros; rows of no group (padding behind the last one) are left as they are
+    in ``out``.  ``scale`` is positive.
 
     ``sink``: fp32 [n_heads], a score per head that joins every softmax denominator (not scaled, not capped, no value);
     ``softcap`` > 0: scores become ``softcap * tanh(score / softcap)`` behind the scale.

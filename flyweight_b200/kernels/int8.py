@@ -21,7 +21,7 @@ from .ops import GATE_ACTIVATIONS
 
 MAX_COLUMNS = 131071          # 128 * 128 * K stays below 2^31
 # up to here the product brings rows to integers by itself, in one launch (one token, 2048 x 2048, with its host time 14.1 -> 11.2 us;
-# every block does it, so with more tokens or columns a launch of its own is faster)
+# every block does it, so with more tokens or columns a launch of its own is faster); the kernel refuses more (int8_product.cuh)
 MAX_RAW, MAX_RAW_COLUMNS = 8, 4096
 _FP32, _BF16 = torch.float32, torch.bfloat16
 
